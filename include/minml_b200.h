@@ -289,6 +289,24 @@ double mb200_probe_mma_cycles(mlContext_t context, int n, int a_in_tensor_memory
 #define MB200_NOALLOC_SCRATCH_BYTES (16u * 1024u * 1024u)
 void mb200_convolution_forward_noalloc(mlContext_t context, mlDataType_t dtype, mlShape_t input_shape, mlShape_t weights_shape, const void *input, const void *weights, void *output, const void *bias, const void *add, mlActivationType_t act);
 
+/* ---- Training and serving of transformer blocks.  None of these has a counterpart in the reference (its layer norm and cross
+ * entropy gradients are declared above as stubs; its host code has no gated block and no loss fused with the output layer).
+ * Common to all: fp16 or fp32 data, dense row-major; the leading extents of a matrix argument may be split ([boards, h, w, channels]
+ * is a matrix of boards * h * w rows).  A descriptor with null data and rank 0 stands for an absent optional operand.  Scratch memory
+ * is the caller's: mb200_*_get_workspace_size tells how much, `workspace` is a descriptor of at least that many bytes, 16-byte aligned,
+ * whose contents need not survive between calls; calls that may overlap on the GPU (two contexts, two replayed graphs) need one each.
+ * No call allocates or synchronises, so each may be captured into a CUDA graph.  Results do not depend on timing (no atomics in sums):
+ * the same call gives the same bits. */
+
+/* Layer normalisation that keeps what its backward pass needs: y as cuda_layernorm_forward, stats [rows, 2] fp32 = (mean, 1 / stddev) of
+ * x + ext.  ext, w, b are optional.  y may be x or ext itself for rows of up to 8192 channels. */
+void mb200_layernorm_forward(mlContext_t context, const mlTensor_t x, const mlTensor_t ext, const mlTensor_t w, const mlTensor_t b, mlTensor_t y, mlTensor_t stats);
+/* dx = gradient of x (and of ext) + beta_dx * dx; dw, db = gradients of weights and bias + beta_dw * their old values, in fp32 or the type of
+ * x.  ext, w, dw, db are optional; dx may be x, ext or dy itself for rows of up to 8192 channels.  With no rows dw and db become
+ * beta_dw * their old values. */
+size_t mb200_layernorm_backward_get_workspace_size(mlContext_t context, mlShape_t shape);
+void mb200_layernorm_backward(mlContext_t context, const mlTensor_t x, const mlTensor_t ext, const mlTensor_t dy, const mlTensor_t w, const mlTensor_t stats, float beta_dx, mlTensor_t dx, float beta_dw, mlTensor_t dw, mlTensor_t db, mlTensor_t workspace);
+
 #ifdef __cplusplus
 }
 #endif

@@ -365,3 +365,23 @@ def fusedBiasActCopyBackward(ctx, dy, y, dx=None, db=None, act="linear", beta_dx
 def activationBackward(ctx, dy, y, dx, act="linear", alpha=1.0, beta=0.0):
     lib.cuda_activation_backward(ctx.handle, alpha, desc(dy, ctx), desc(y, ctx), beta, desc(dx, ctx), act_code(act))
     ctx.check()
+
+
+# ---------------------------------------------------------------------------------------------- training and serving of transformer blocks
+# (extensions: the reference has no counterpart; the C declarations in include/minml_b200.h say what each argument means)
+def layernormForwardTraining(ctx, x, y, weights, bias, stats, ext=None):
+    """layernormForward that also writes stats (fp32 [rows, 2]: mean and 1 / stddev of every row) for layernormBackward."""
+    lib.mb200_layernorm_forward(ctx.handle, desc(x, ctx), desc(ext, ctx), desc(weights, ctx), desc(bias, ctx), desc(y, ctx), desc(stats, ctx))
+    ctx.check()
+
+
+def layernormBackwardGetWorkspaceSize(ctx, x_shape):
+    """Bytes of scratch memory layernormBackward needs for an input of this shape."""
+    return lib.mb200_layernorm_backward_get_workspace_size(ctx.handle, shape_of(x_shape))
+
+
+def layernormBackward(ctx, x, dy, dx, weights, stats, dw=None, db=None, ext=None, beta_dx=0.0, beta_dw=0.0, workspace=None):
+    """dx = gradient of x (and of ext) + beta_dx * dx; dw, db (fp32 or x's type) = gradients + beta_dw * old values, reduced in a fixed order."""
+    lib.mb200_layernorm_backward(ctx.handle, desc(x, ctx), desc(ext, ctx), desc(dy, ctx), desc(weights, ctx), desc(stats, ctx), beta_dx, desc(dx, ctx), beta_dw,
+                                 desc(dw, ctx), desc(db, ctx), desc(workspace, ctx))
+    ctx.check()
