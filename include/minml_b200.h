@@ -307,6 +307,30 @@ void mb200_layernorm_forward(mlContext_t context, const mlTensor_t x, const mlTe
 size_t mb200_layernorm_backward_get_workspace_size(mlContext_t context, mlShape_t shape);
 void mb200_layernorm_backward(mlContext_t context, const mlTensor_t x, const mlTensor_t ext, const mlTensor_t dy, const mlTensor_t w, const mlTensor_t stats, float beta_dx, mlTensor_t dx, float beta_dw, mlTensor_t dw, mlTensor_t db, mlTensor_t workspace);
 
+/* Gated feed-forward block: y = (act(x Wg^T) * (x Wu^T)) W2^T + beta * y with W1 = [Wg; Wu], a [2 hidden, embed] matrix (gate rows first), and
+ * W2 [embed, hidden].  `gate` names act.  `saved` (optional, fp32 [tokens, 2 hidden]) is where the forward pass may leave what its backward
+ * pass reads instead of computing it again; its contents are the library's own. */
+#define MB200_GATE_SIGMOID 0
+#define MB200_GATE_RELU 1
+#define MB200_GATE_SILU 2
+#define MB200_GATE_GELU 3
+/* Workspace of the forward call (training = false) or of the forward and the backward call, with or without `saved`. */
+size_t mb200_gated_feed_forward_get_workspace_size(mlContext_t context, mlShape_t x_shape, mlShape_t w1_shape, mlDataType_t dtype, bool training, bool saved);
+void mb200_gated_feed_forward_forward(mlContext_t context, const mlTensor_t x, const mlTensor_t w1, const mlTensor_t w2, float beta, mlTensor_t y, int gate, mlTensor_t saved, mlTensor_t workspace);
+/* Gradients for dy, each + beta times its old value; dx, dw1, dw2 are optional.  `saved` is the forward call's (same x, w1 and gate), or absent:
+ * what it would hold is then computed again. */
+void mb200_gated_feed_forward_backward(mlContext_t context, const mlTensor_t x, const mlTensor_t w1, const mlTensor_t w2, const mlTensor_t saved, const mlTensor_t dy, float beta_dx, mlTensor_t dx, float beta_dw, mlTensor_t dw1, mlTensor_t dw2, int gate, mlTensor_t workspace);
+
+/* Softmax cross entropy of the logits x W^T (W [vocabulary, embed]) without keeping them: loss[t] = log sum_v exp(x_t . w_v) - x_t . w_target,
+ * fp32; lse (optional, fp32 [tokens]) receives the first term for the backward pass.  targets: int32 [tokens]; a value outside
+ * [0, vocabulary) leaves the row out: loss 0, no gradient.  The workspace decides how wide a piece of the vocabulary is taken at a
+ * time: the size asked for is a good one, less (down to pieces of 256 columns) costs some speed. */
+size_t mb200_softmax_cross_entropy_get_workspace_size(mlContext_t context, mlShape_t x_shape, mlShape_t w_shape, mlDataType_t dtype, bool training);
+void mb200_softmax_cross_entropy_forward(mlContext_t context, const mlTensor_t x, const mlTensor_t w, const mlTensor_t targets, mlTensor_t loss, mlTensor_t lse, mlTensor_t workspace);
+/* Gradients of alpha * sum_t row_weights[t] * loss[t] (row_weights optional, fp32 [tokens]), each + beta times its old value; dx, dw are
+ * optional.  A row of weight 0 is left out like one without a target.  fp16: choose alpha (the loss scale) so that the gradients fit. */
+void mb200_softmax_cross_entropy_backward(mlContext_t context, const mlTensor_t x, const mlTensor_t w, const mlTensor_t targets, const mlTensor_t lse, float alpha, const mlTensor_t row_weights, float beta_dx, mlTensor_t dx, float beta_dw, mlTensor_t dw, mlTensor_t workspace);
+
 #ifdef __cplusplus
 }
 #endif

@@ -385,3 +385,53 @@ def layernormBackward(ctx, x, dy, dx, weights, stats, dw=None, db=None, ext=None
     lib.mb200_layernorm_backward(ctx.handle, desc(x, ctx), desc(ext, ctx), desc(dy, ctx), desc(weights, ctx), desc(stats, ctx), beta_dx, desc(dx, ctx), beta_dw,
                                  desc(dw, ctx), desc(db, ctx), desc(workspace, ctx))
     ctx.check()
+
+
+GATES = {"sigmoid": 0, "relu": 1, "silu": 2, "gelu": 3}
+
+
+def gate_code(gate):
+    if gate not in GATES:
+        raise BackendError("unknown gate %r: one of %s" % (gate, ", ".join(sorted(GATES))))
+    return GATES[gate]
+
+
+def _floating(dtype):
+    if dtype not in _DTYPES:
+        raise BackendError("unsupported type %s" % dtype)
+    return _DTYPES[dtype]
+
+
+def gatedFeedForwardGetWorkspaceSize(ctx, x_shape, w1_shape, dtype=torch.float16, training=False, saved=True):
+    """Bytes of scratch memory for the forward call or, training, for both calls; saved=False: the backward call gets no `saved` tensor."""
+    return lib.mb200_gated_feed_forward_get_workspace_size(ctx.handle, shape_of(x_shape), shape_of(w1_shape), _floating(dtype), bool(training), bool(training and saved))
+
+
+def gatedFeedForwardForward(ctx, x, w1, w2, y, gate="silu", beta=0.0, saved=None, workspace=None):
+    """y = (act(x Wg^T) * (x Wu^T)) W2^T + beta * y, w1 = [Wg; Wu] of shape [2 hidden, embed], w2 of shape [embed, hidden]."""
+    lib.mb200_gated_feed_forward_forward(ctx.handle, desc(x, ctx), desc(w1, ctx), desc(w2, ctx), beta, desc(y, ctx), gate_code(gate), desc(saved, ctx), desc(workspace, ctx))
+    ctx.check()
+
+
+def gatedFeedForwardBackward(ctx, x, w1, w2, dy, dx=None, dw1=None, dw2=None, gate="silu", saved=None, beta_dx=0.0, beta_dw=0.0, workspace=None):
+    """Gradients of gatedFeedForwardForward for dy; `saved` is the tensor given to the forward call, or None (then it is computed again)."""
+    lib.mb200_gated_feed_forward_backward(ctx.handle, desc(x, ctx), desc(w1, ctx), desc(w2, ctx), desc(saved, ctx), desc(dy, ctx), beta_dx, desc(dx, ctx), beta_dw,
+                                          desc(dw1, ctx), desc(dw2, ctx), gate_code(gate), desc(workspace, ctx))
+    ctx.check()
+
+
+def softmaxCrossEntropyGetWorkspaceSize(ctx, x_shape, w_shape, dtype=torch.float16, training=False):
+    return lib.mb200_softmax_cross_entropy_get_workspace_size(ctx.handle, shape_of(x_shape), shape_of(w_shape), _floating(dtype), bool(training))
+
+
+def softmaxCrossEntropyForward(ctx, x, weights, targets, loss, lse=None, workspace=None):
+    """loss[t] = log sum_v exp(x_t . w_v) - x_t . w_target (fp32), 0 for a target outside the vocabulary; lse[t] keeps the first term."""
+    lib.mb200_softmax_cross_entropy_forward(ctx.handle, desc(x, ctx), desc(weights, ctx), desc(targets, ctx), desc(loss, ctx), desc(lse, ctx), desc(workspace, ctx))
+    ctx.check()
+
+
+def softmaxCrossEntropyBackward(ctx, x, weights, targets, lse, dx=None, dw=None, alpha=1.0, row_weights=None, beta_dx=0.0, beta_dw=0.0, workspace=None):
+    """Gradients of alpha * sum_t row_weights[t] * loss[t], each + beta times its old value."""
+    lib.mb200_softmax_cross_entropy_backward(ctx.handle, desc(x, ctx), desc(weights, ctx), desc(targets, ctx), desc(lse, ctx), alpha, desc(row_weights, ctx), beta_dx, desc(dx, ctx),
+                                             beta_dw, desc(dw, ctx), desc(workspace, ctx))
+    ctx.check()
