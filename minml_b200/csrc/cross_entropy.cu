@@ -12,9 +12,16 @@
  * fp16 gradients: P reaches down to 1 / vocabulary, where fp16 has left its normal range, so it is rounded as 2^15 P (at most 32768;
  * relative precision down to 2^-29).  Row weights do not go into P, where small ones would cost dx its digits, but into dx's fp32
  * result and into a copy of x, as c_t / max |c| (exact where all weights are equal).
+ *
+ * fp16 runs on gemm_pair.cu: forward is one product whose epilogue leaves (maximum, sum of exponentials) for every row and 128 columns,
+ * joined by a second kernel, and the whole vocabulary is one piece; backward makes 2^15 P of a piece in the epilogue of its logits and
+ * multiplies it with W and x.  dx is added up over the pieces in fp32.  fp32 keeps one piece's logits.  An embed that is no multiple of 16
+ * bytes is copied to padded rows first.
  */
 #include "common.cuh"
 #include "operands.cuh"
+#include "gemm_pair.cuh"
+#include "gemm_fp32.cuh"
 
 #include <algorithm>
 
@@ -68,13 +75,13 @@ namespace mb200
 		}
 
 		/* One block a row: joins the piece's columns [first, first + width) into the row's running maximum and sum. */
-		__global__ void __launch_bounds__(256) kernel_piece_statistics(const float *__restrict__ z, float2 *__restrict__ running, float *__restrict__ target_logit, Rows rows,
+		__global__ void __launch_bounds__(256) kernel_piece_statistics(const float *__restrict__ z, int pitch, float2 *__restrict__ running, float *__restrict__ target_logit, Rows rows,
 				long long tokens, int first, int width, bool last, float *__restrict__ loss, float *__restrict__ lse)
 		{
 			__shared__ float2 scratch[8];
 			for (long long t = blockIdx.x; t < tokens; t += gridDim.x)
 			{
-				const float *row = z + t * width;
+				const float *row = z + t * pitch;
 				float2 mine = make_float2(-INFINITY, 0.0f);
 				for (int c = threadIdx.x; c < width; c += 256)
 				{
@@ -108,18 +115,16 @@ namespace mb200
 			}
 		}
 
-		/* p = scale (exp(z - lse) - [target]) for one piece; rows that take no part are zero */
-		template<typename T>
-		__global__ void __launch_bounds__(256) kernel_piece_gradient(T *__restrict__ p, const float *__restrict__ z, const float *__restrict__ lse, Rows rows, long long tokens,
-				int first, int width, float scale)
+		/* z becomes exp(z - lse) - [target] for one piece; rows that take no part are zero */
+		__global__ void __launch_bounds__(256) kernel_piece_gradient(float *__restrict__ z, int pitch, const float *__restrict__ lse, Rows rows, long long tokens, int first, int width)
 		{
 			const long long total = tokens * width, stride = static_cast<long long>(gridDim.x) * 256;
 			for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < total; i += stride)
 			{
 				const long long t = i / width;
 				const int c = static_cast<int>(i - t * width);
-				const float v = expf(z[i] - lse[t]) - (rows.targets[t] - first == c ? 1.0f : 0.0f);
-				p[i] = from_float<T>(rows.weight(t) != 0.0f ? scale * v : 0.0f);
+				const float v = expf(z[t * pitch + c] - lse[t]) - (rows.targets[t] - first == c ? 1.0f : 0.0f);
+				z[t * pitch + c] = rows.weight(t) != 0.0f ? v : 0.0f;
 			}
 		}
 
@@ -156,25 +161,26 @@ namespace mb200
 					out[t * embed + k] = factor == 0.0f ? from_float<T>(0.0f) : from_float<T>(to_float(x[t * embed + k]) * factor);
 			}
 		}
-		/* out = alpha * (largest) * (row weight) * sum + beta * out, the rounding of an fp32 sum to the gradient's type */
-		template<typename T>
-		__global__ void __launch_bounds__(256) kernel_finish_gradient(T *out, const float *__restrict__ sum, float alpha, const float *__restrict__ largest, const float *__restrict__ row_weights,
-				float beta, long long elements, int columns)
+		/* Joins the groups' statistics of a row: a block takes 32 rows, its 32 warps every 32nd group. */
+		__global__ void __launch_bounds__(1024) kernel_join_statistics(const float2 *__restrict__ parts, int groups, const float *__restrict__ target_logit, Rows rows, long long tokens,
+				float *__restrict__ loss, float *__restrict__ lse)
 		{
-			const long long stride = static_cast<long long>(gridDim.x) * 256;
-			const float factor = largest == nullptr ? alpha : alpha * largest[0];
-			for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < elements; i += stride)
-			{
-				const float c = row_weights == nullptr ? 1.0f : row_weights[i / columns];
-				const float v = c == 0.0f ? 0.0f : factor * c * sum[i]; // a sum of a row that takes no part is zero already
-				out[i] = from_float<T>(beta != 0.0f ? v + beta * to_float(out[i]) : v);
-			}
+			__shared__ float2 scratch[32][33];
+			const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+			const long long t = static_cast<long long>(blockIdx.x) * 32 + lane;
+			wait_for_previous_grid();
+			float2 mine = make_float2(-INFINITY, 0.0f);
+			if (t < tokens)
+				for (int g = warp; g < groups; g += 32)
+					mine = merge(mine, parts[g * tokens + t]);
+			scratch[lane][warp] = mine;
+			__syncthreads();
+			const float2 total = merge_warp(scratch[warp][lane]);
+			const long long row = static_cast<long long>(blockIdx.x) * 32 + warp;
+			if (lane == 0 && row < tokens)
+				finish_row(row, total, rows, target_logit, loss, lse);
 		}
 
-		mlTensor_t matrix(const void *data, mlDataType_t dtype, long long rows, int columns)
-		{
-			return make_tensor(data, dtype, make_shape( { static_cast<int>(rows), columns }));
-		}
 		int elementwise_blocks(mlContext_t ctx, long long elements)
 		{
 			return static_cast<int>(std::max<long long>(1, std::min<long long>((elements + 255) / 256, static_cast<long long>(get(ctx)->sm_count) * 8)));
@@ -185,49 +191,75 @@ namespace mb200
 		}
 
 		/* The workspace of one call with pieces of `piece` columns. */
-		struct Scratch
+		struct Plan
 		{
-				float2 *running = nullptr;
-				float *target_logit = nullptr, *z = nullptr, *dx_sum = nullptr, *dw_sum = nullptr, *largest = nullptr;
-				void *p = nullptr, *x = nullptr;
+				int embed; // padded to a pitch that TMA can address
+				int piece, pitch; // columns of a piece of logits or probabilities, and its rows' pitch
+				int dx_splits; // fp32 sums that dx is kept in until the last piece
+				float2 *running = nullptr; // fp32: per row; fp16: per row and 128 columns
+				float *target_logit = nullptr, *z = nullptr, *dx_sums = nullptr, *partials = nullptr, *largest = nullptr;
+				void *p = nullptr, *x = nullptr, *w = nullptr, *weighted_x = nullptr;
 				size_t bytes = 0;
-				Scratch(const Problem &q, void *workspace, bool training, int piece)
+				Plan(mlContext_t ctx, const Problem &q, void *workspace, bool training, int columns)
 				{
 					Carver carve(workspace);
-					const size_t es = size_of(q.dtype), cells = static_cast<size_t>(q.tokens) * piece, rows = static_cast<size_t>(q.tokens) * q.embed;
-					running = carve.take<float2>(q.tokens);
-					target_logit = carve.take<float>(q.tokens);
-					z = carve.take<float>(cells);
+					const bool half = q.dtype == DTYPE_FLOAT16;
+					const int es = size_of(q.dtype), tokens = static_cast<int>(q.tokens);
+					embed = round_up(q.embed, 16 / es);
+					piece = columns;
+					pitch = round_up(columns, 64);
+					dx_splits = half && training ? pair_splits(ctx, tokens, q.embed, piece) : 1;
+					const size_t cells = static_cast<size_t>(q.tokens) * pitch, rows = static_cast<size_t>(q.tokens) * embed;
+					if (embed != q.embed)
+					{
+						x = carve.take<uint8_t>(rows * es);
+						w = carve.take<uint8_t>(static_cast<size_t>(q.vocab) * embed * es);
+					}
+					if (!training)
+					{
+						target_logit = carve.take<float>(q.tokens);
+						running = carve.take<float2>(q.tokens * (half ? pair_statistics_parts(q.vocab) : 1));
+					}
+					if (!half)
+						z = carve.take<float>(cells);
 					if (training)
 					{
 						largest = carve.take<float>(1);
-						x = carve.take<uint8_t>(rows * es);
-						dx_sum = carve.take<float>(rows);
-						p = carve.take<uint8_t>(cells * es);
-						dw_sum = carve.take<float>(static_cast<size_t>(piece) * q.embed);
+						weighted_x = carve.take<uint8_t>(rows * es);
+						p = half ? carve.take<uint8_t>(cells * es) : nullptr; // fp32: in place of the logits
+						dx_sums = carve.take<float>(rows * dx_splits);
+						// dW of a piece: fp16 may be cut along K, fp32 goes through a sum so that a device-side factor can be applied
+						const int last = q.vocab - (q.vocab - 1) / piece * piece;
+						partials = carve.take<float>(half ? std::max(pair_partial_elements(ctx, piece, q.embed, tokens), pair_partial_elements(ctx, last, q.embed, tokens))
+								: static_cast<size_t>(piece) * embed);
 					}
 					bytes = carve.used;
 				}
 		};
-		int recommended_piece(const Problem &q)
-		{
-			const long long columns = static_cast<long long>(PIECE_BYTES / 4) / std::max<long long>(1, q.tokens) / 64 * 64;
-			return static_cast<int>(std::min<long long>(q.vocab, std::max<long long>(MIN_PIECE, columns)));
+		bool in_pieces(const Problem &q, bool training)
+		{ // the forward pass in fp16 keeps 8 bytes for every row and 128 columns and has no use for pieces
+			return training || q.dtype == DTYPE_FLOAT32;
 		}
-		/* The widest piece, a multiple of 64 columns or the whole vocabulary, whose scratch fits the workspace; 0 if none does. */
-		int piece_that_fits(const Problem &q, bool training, size_t bytes)
+		/* Pieces of equal width, multiples of 256 columns, of at most about PIECE_BYTES. */
+		int recommended_piece(const Problem &q, bool training)
 		{
-			if (Scratch(q, nullptr, training, q.vocab).bytes <= bytes)
+			if (!in_pieces(q, training))
 				return q.vocab;
-			int low = std::min(MIN_PIECE, q.vocab), high = q.vocab; // low fits (checked), high does not
-			if (Scratch(q, nullptr, training, low).bytes > bytes)
-				return 0;
-			while (high - low > 64)
-			{
-				const int middle = low + (high - low) / 2;
-				(Scratch(q, nullptr, training, middle).bytes <= bytes ? low : high) = middle;
-			}
-			return std::max(std::min(MIN_PIECE, q.vocab), low / 64 * 64);
+			const long long most = std::max<long long>(MIN_PIECE, static_cast<long long>(PIECE_BYTES / size_of(q.dtype)) / std::max<long long>(1, q.tokens));
+			const long long pieces = (q.vocab + most - 1) / most;
+			return static_cast<int>(std::min<long long>(q.vocab, round_up(static_cast<int>((q.vocab + pieces - 1) / pieces), 256)));
+		}
+		/* The widest piece up to the recommended one, a multiple of 64 columns or the whole vocabulary, whose scratch fits the workspace; 0 if
+		 * none does. */
+		int piece_that_fits(mlContext_t ctx, const Problem &q, bool training, size_t bytes)
+		{
+			const int best = recommended_piece(q, training);
+			if (Plan(ctx, q, nullptr, training, best).bytes <= bytes)
+				return best;
+			for (int piece = best / 2 / 64 * 64; piece > MIN_PIECE; piece = piece * 3 / 4 / 64 * 64)
+				if (Plan(ctx, q, nullptr, training, piece).bytes <= bytes)
+					return piece;
+			return Plan(ctx, q, nullptr, training, std::min(MIN_PIECE, best)).bytes <= bytes ? std::min(MIN_PIECE, best) : 0;
 		}
 
 		bool check_problem(mlContext_t ctx, const char *who, const mlTensor_t &x, const mlTensor_t &w, const mlTensor_t &targets, Problem &q)
@@ -256,61 +288,123 @@ namespace mb200
 			return check_operand(ctx, who, "x", x, x.dtype, q.tokens, q.embed) && check_operand(ctx, who, "weights", w, x.dtype, q.vocab, q.embed)
 					&& check_operand(ctx, who, "targets", targets, DTYPE_INT32, q.tokens);
 		}
+		/* Width of the pieces for this workspace; 0 (and an error) when it holds none. */
 		int check_piece(mlContext_t ctx, const char *who, const Problem &q, bool training, const mlTensor_t &workspace)
 		{
-			const size_t least = Scratch(q, nullptr, training, std::min(MIN_PIECE, q.vocab)).bytes;
-			if (!check_workspace(ctx, who, workspace, least))
+			if (!check_workspace(ctx, who, workspace, 1))
 				return 0;
-			return piece_that_fits(q, training, static_cast<size_t>(bytes_of(workspace)));
-		}
-		mlTensor_t piece_of(const mlTensor_t &w, int first, int width)
-		{
-			return matrix(reinterpret_cast<const uint8_t*>(w.data) + static_cast<size_t>(first) * w.dim[1] * size_of(w.dtype), w.dtype, width, w.dim[1]);
+			const int piece = piece_that_fits(ctx, q, training, static_cast<size_t>(bytes_of(workspace)));
+			if (piece == 0)
+				record_error(ctx, "%s: the workspace has %lld bytes, %zu are needed", who, bytes_of(workspace),
+						Plan(ctx, q, nullptr, training, std::min(MIN_PIECE, recommended_piece(q, training))).bytes);
+			return piece;
 		}
 		template<typename T>
-		void backward_pieces(mlContext_t ctx, const Problem &q, const Rows &rows, const mlTensor_t &x, const mlTensor_t &w, const float *lse, float alpha, float beta_dx,
-				const mlTensor_t &dx, float beta_dw, const mlTensor_t &dw, const Scratch &s, int piece)
+		struct Operands
+		{
+				const T *x, *w;
+				Operands(mlContext_t ctx, const Problem &q, const Plan &plan, const mlTensor_t &x_, const mlTensor_t &w_) :
+						x(reinterpret_cast<const T*>(x_.data)),
+						w(reinterpret_cast<const T*>(w_.data))
+				{
+					if (plan.x != nullptr)
+					{
+						pack_rows<T>(ctx, reinterpret_cast<T*>(plan.x), plan.embed, q.tokens, x, q.tokens, q.embed);
+						pack_rows<T>(ctx, reinterpret_cast<T*>(plan.w), plan.embed, q.vocab, w, q.vocab, q.embed);
+						x = reinterpret_cast<const T*>(plan.x);
+						w = reinterpret_cast<const T*>(plan.w);
+					}
+				}
+		};
+		bool check_alignment(mlContext_t ctx, const char *who, const char *name, const mlTensor_t &t, bool copied)
+		{
+			if (copied || aligned_to(t.data, 16))
+				return true;
+			record_error(ctx, "%s: %s must be 16-byte aligned", who, name);
+			return false;
+		}
+
+		void forward_half(mlContext_t ctx, const Problem &q, const Rows &rows, const Plan &plan, const Operands<__half> &o, float *loss, float *lse)
+		{
+			if (!pair_statistics(ctx, static_cast<int>(q.tokens), q.vocab, q.embed, PairOperand { o.x, plan.embed, false }, PairOperand { o.w, plan.embed, false }, rows.targets,
+					plan.running, plan.target_logit))
+				return;
+			const cudaError_t status = launch_overlapped(kernel_join_statistics, dim3(static_cast<unsigned>((q.tokens + 31) / 32)), dim3(1024), 0, use_stream(ctx), plan.running,
+					pair_statistics_parts(q.vocab), plan.target_logit, rows, q.tokens, loss, lse);
+			MB200_COUNT_LAUNCH();
+			check_cuda(ctx, status, "mb200_softmax_cross_entropy_forward");
+		}
+		void forward_float(mlContext_t ctx, const Problem &q, const Rows &rows, const Plan &plan, const Operands<float> &o, float *loss, float *lse)
+		{
+			for (int first = 0; first < q.vocab; first += plan.piece)
+			{
+				const int width = std::min(plan.piece, q.vocab - first);
+				if (!float_product(ctx, static_cast<int>(q.tokens), width, q.embed, FloatOperand { o.x, plan.embed, false },
+						FloatOperand { o.w + static_cast<size_t>(first) * plan.embed, plan.embed, false }, plan.z, plan.pitch, 1.0f, 0.0f))
+					return;
+				kernel_piece_statistics<<<row_blocks(ctx, q.tokens), 256, 0, use_stream(ctx)>>>(plan.z, plan.pitch, plan.running, plan.target_logit, rows, q.tokens, first, width,
+						first + width == q.vocab, loss, lse);
+				MB200_COUNT_LAUNCH();
+			}
+			check_cuda(ctx, cudaGetLastError(), "mb200_softmax_cross_entropy_forward");
+		}
+		template<typename T>
+		void backward(mlContext_t ctx, const Problem &q, const Rows &rows, const Plan &plan, const Operands<T> &o, const float *lse, float alpha, float beta_dx, T *dx, float beta_dw, T *dw)
 		{
 			cudaStream_t stream = use_stream(ctx);
-			const float scale = q.dtype == DTYPE_FLOAT16 ? P_SCALE : 1.0f;
-			const bool want_dx = !is_empty_descriptor(dx), want_dw = !is_empty_descriptor(dw);
-			const float *largest = rows.weights == nullptr ? nullptr : s.largest;
-			if (largest != nullptr)
+			constexpr bool half = sizeof(T) == 2;
+			const int tokens = static_cast<int>(q.tokens), D = q.embed, ld = plan.embed;
+			const float unscale = half ? alpha / P_SCALE : alpha;
+			const float *largest = rows.weights == nullptr ? nullptr : plan.largest;
+			if (dw != nullptr)
 			{
-				kernel_largest_weight<<<1, 1024, 0, stream>>>(s.largest, rows, q.tokens);
-				MB200_COUNT_LAUNCH();
-			}
-			if (want_dw)
-			{
-				kernel_weighted_rows<T> <<<row_blocks(ctx, q.tokens), 256, 0, stream>>>(reinterpret_cast<T*>(s.x), reinterpret_cast<const T*>(x.data), rows, largest, q.tokens, q.embed);
-				MB200_COUNT_LAUNCH();
-			}
-			const mlTensor_t x2 = matrix(x.data, q.dtype, q.tokens, q.embed), dx_sum = matrix(s.dx_sum, DTYPE_FLOAT32, q.tokens, q.embed);
-			for (int first = 0; first < q.vocab; first += piece)
-			{
-				const int width = std::min(piece, q.vocab - first);
-				const mlTensor_t wp = piece_of(w, first, width), p = matrix(s.p, q.dtype, q.tokens, width);
-				cuda_gemm_v2(ctx, 'n', 't', 1.0f, x2, wp, 0.0f, matrix(s.z, DTYPE_FLOAT32, q.tokens, width));
-				kernel_piece_gradient<T> <<<elementwise_blocks(ctx, q.tokens * width), 256, 0, stream>>>(reinterpret_cast<T*>(s.p), s.z, lse, rows, q.tokens, first, width, scale);
-				MB200_COUNT_LAUNCH();
-				if (want_dx)
-					cuda_gemm_v2(ctx, 'n', 'n', 1.0f, p, wp, first == 0 ? 0.0f : 1.0f, dx_sum);
-				if (want_dw)
+				if (largest != nullptr)
 				{
-					cuda_gemm_v2(ctx, 't', 'n', 1.0f, p, matrix(s.x, q.dtype, q.tokens, q.embed), 0.0f, matrix(s.dw_sum, DTYPE_FLOAT32, width, q.embed));
-					const long long n = static_cast<long long>(width) * q.embed;
-					kernel_finish_gradient<T> <<<elementwise_blocks(ctx, n), 256, 0, stream>>>(reinterpret_cast<T*>(dw.data) + static_cast<size_t>(first) * q.embed, s.dw_sum, alpha / scale,
-							largest, nullptr, beta_dw, n, q.embed);
+					kernel_largest_weight<<<1, 1024, 0, stream>>>(plan.largest, rows, q.tokens);
 					MB200_COUNT_LAUNCH();
 				}
-			}
-			if (want_dx)
-			{
-				const long long n = q.tokens * q.embed;
-				kernel_finish_gradient<T> <<<elementwise_blocks(ctx, n), 256, 0, stream>>>(reinterpret_cast<T*>(dx.data), s.dx_sum, alpha / scale, nullptr, rows.weights, beta_dx, n, q.embed);
+				kernel_weighted_rows<T> <<<row_blocks(ctx, q.tokens), 256, 0, stream>>>(reinterpret_cast<T*>(plan.weighted_x), o.x, rows, largest, q.tokens, ld);
 				MB200_COUNT_LAUNCH();
+				if (!check_cuda(ctx, cudaGetLastError(), "mb200_softmax_cross_entropy_backward: row weights"))
+					return;
 			}
-			check_cuda(ctx, cudaGetLastError(), "mb200_softmax_cross_entropy_backward");
+			const T *weighted_x = reinterpret_cast<const T*>(plan.weighted_x);
+			for (int first = 0; first < q.vocab; first += plan.piece)
+			{
+				const int width = std::min(plan.piece, q.vocab - first);
+				const T *w = o.w + static_cast<size_t>(first) * ld;
+				if constexpr (half)
+				{
+					__half *p = reinterpret_cast<__half*>(plan.p);
+					if (!pair_probabilities(ctx, tokens, width, D, PairOperand { o.x, ld, false }, PairOperand { w, ld, false }, rows.targets, rows.weights, lse, first, q.vocab, p, plan.pitch))
+						return;
+					if (dx != nullptr
+							&& !pair_product_sums(ctx, tokens, D, width, PairOperand { p, plan.pitch, false }, PairOperand { w, ld, true }, plan.dx_sums, ld, plan.dx_splits, first > 0))
+						return;
+					if (dw != nullptr
+							&& !pair_product(ctx, width, D, tokens, PairOperand { p, plan.pitch, true }, PairOperand { weighted_x, ld, true },
+									PairResult { dw + static_cast<size_t>(first) * D, D, unscale, beta_dw, largest }, plan.partials))
+						return;
+				}
+				else
+				{
+					if (!float_product(ctx, tokens, width, D, FloatOperand { o.x, ld, false }, FloatOperand { w, ld, false }, plan.z, plan.pitch, 1.0f, 0.0f))
+						return;
+					kernel_piece_gradient<<<elementwise_blocks(ctx, q.tokens * width), 256, 0, stream>>>(plan.z, plan.pitch, lse, rows, q.tokens, first, width);
+					MB200_COUNT_LAUNCH();
+					if (!check_cuda(ctx, cudaGetLastError(), "mb200_softmax_cross_entropy_backward: probabilities"))
+						return;
+					if (dx != nullptr
+							&& !float_product(ctx, tokens, D, width, FloatOperand { plan.z, plan.pitch, false }, FloatOperand { w, ld, true }, plan.dx_sums, ld, 1.0f, first > 0 ? 1.0f : 0.0f))
+						return;
+					if (dw != nullptr
+							&& (!float_product(ctx, width, D, tokens, FloatOperand { plan.z, plan.pitch, true }, FloatOperand { weighted_x, ld, true }, plan.partials, ld, 1.0f, 0.0f)
+									|| !finish_sums<float>(ctx, dw + static_cast<size_t>(first) * D, D, width, D, plan.partials, ld, 1, unscale, largest, nullptr, beta_dw)))
+						return;
+				}
+			}
+			if (dx != nullptr)
+				finish_sums<T>(ctx, dx, D, tokens, D, plan.dx_sums, ld, plan.dx_splits, unscale, nullptr, rows.weights, beta_dx);
 		}
 	}
 } /* namespace mb200 */
@@ -324,7 +418,11 @@ extern "C"
 		if (context == nullptr || x_shape.rank < 1 || x_shape.rank > 6 || w_shape.rank != 2 || w_shape.dim[0] <= 0 || w_shape.dim[1] <= 0 || last_dim(x_shape) != w_shape.dim[1])
 			return 0;
 		const Problem q { dtype, volume_without_last_dim(x_shape), w_shape.dim[1], w_shape.dim[0] };
-		return q.tokens <= 0 ? 0 : Scratch(q, nullptr, training, recommended_piece(q)).bytes;
+		if (q.tokens <= 0 || q.tokens > 0x7FFFFFFFll || (dtype != DTYPE_FLOAT16 && dtype != DTYPE_FLOAT32))
+			return 0;
+		// the forward call of a training step takes its scratch from the same workspace
+		const size_t forward = Plan(context, q, nullptr, false, recommended_piece(q, false)).bytes;
+		return training ? std::max(forward, Plan(context, q, nullptr, true, recommended_piece(q, true)).bytes) : forward;
 	}
 
 	void mb200_softmax_cross_entropy_forward(mlContext_t context, const mlTensor_t x, const mlTensor_t w, const mlTensor_t targets, mlTensor_t loss, mlTensor_t lse, mlTensor_t workspace)
@@ -351,19 +449,16 @@ extern "C"
 		const int piece = check_piece(context, who, q, false, workspace);
 		if (piece == 0)
 			return;
+		const Plan plan(context, q, workspace.data, false, piece);
+		if (!check_alignment(context, who, "x", x, plan.x != nullptr) || !check_alignment(context, who, "weights", w, plan.x != nullptr))
+			return;
 		flush_pending(context);
-		const Scratch s(q, workspace.data, false, piece);
 		const Rows rows { reinterpret_cast<const int*>(targets.data), nullptr, q.vocab };
-		const mlTensor_t x2 = matrix(x.data, q.dtype, q.tokens, q.embed);
-		for (int first = 0; first < q.vocab; first += piece)
-		{
-			const int width = std::min(piece, q.vocab - first);
-			cuda_gemm_v2(context, 'n', 't', 1.0f, x2, piece_of(w, first, width), 0.0f, matrix(s.z, DTYPE_FLOAT32, q.tokens, width));
-			kernel_piece_statistics<<<row_blocks(context, q.tokens), 256, 0, use_stream(context)>>>(s.z, s.running, s.target_logit, rows, q.tokens, first, width,
-					first + width == q.vocab, reinterpret_cast<float*>(loss.data), reinterpret_cast<float*>(lse.data));
-			MB200_COUNT_LAUNCH();
-		}
-		check_cuda(context, cudaGetLastError(), who);
+		float *loss_data = reinterpret_cast<float*>(loss.data), *lse_data = reinterpret_cast<float*>(lse.data);
+		if (q.dtype == DTYPE_FLOAT16)
+			forward_half(context, q, rows, plan, Operands<__half>(context, q, plan, x, w), loss_data, lse_data);
+		else
+			forward_float(context, q, rows, plan, Operands<float>(context, q, plan, x, w), loss_data, lse_data);
 	}
 
 	void mb200_softmax_cross_entropy_backward(mlContext_t context, const mlTensor_t x, const mlTensor_t w, const mlTensor_t targets, const mlTensor_t lse, float alpha,
@@ -398,12 +493,16 @@ extern "C"
 		const int piece = check_piece(context, who, q, true, workspace);
 		if (piece == 0)
 			return;
-		const Scratch s(q, workspace.data, true, piece);
+		const Plan plan(context, q, workspace.data, true, piece);
+		if (!check_alignment(context, who, "x", x, plan.x != nullptr) || !check_alignment(context, who, "weights", w, plan.x != nullptr))
+			return;
 		const Rows rows { reinterpret_cast<const int*>(targets.data), reinterpret_cast<const float*>(row_weights.data), q.vocab };
 		const float *lse_data = reinterpret_cast<const float*>(lse.data);
 		if (q.dtype == DTYPE_FLOAT16)
-			backward_pieces<__half>(context, q, rows, x, w, lse_data, alpha, beta_dx, dx, beta_dw, dw, s, piece);
+			backward<__half>(context, q, rows, plan, Operands<__half>(context, q, plan, x, w), lse_data, alpha, beta_dx, reinterpret_cast<__half*>(dx.data), beta_dw,
+					reinterpret_cast<__half*>(dw.data));
 		else
-			backward_pieces<float>(context, q, rows, x, w, lse_data, alpha, beta_dx, dx, beta_dw, dw, s, piece);
+			backward<float>(context, q, rows, plan, Operands<float>(context, q, plan, x, w), lse_data, alpha, beta_dx, reinterpret_cast<float*>(dx.data), beta_dw,
+					reinterpret_cast<float*>(dw.data));
 	}
 }

@@ -5,10 +5,17 @@
  * u = x Wu^T, h = act(a) u and dh = dy W2:
  *   da = dh u act'(a);   du = dh act(a);   dx = [da du] W1;   dW1 = [da du]^T x;   dW2 = dy^T h
  * 6 T D F operations forward and 12 backward; a few tokens are bound by reading the 3 D F weights instead.
+ *
+ * fp16: two launches forward (gemm_pair.cu): the first product's tile holds 128 gate and the matching 128 up columns, so its epilogue
+ * writes h alone; backward four, [da du] and h coming out of the product that makes dh.  h, da, du are rounded to fp16 once, a and u
+ * reach the backward pass in fp32 (rounded to fp16 they would double its error).  fp32: five and eight launches, with the gate between.
+ * Extents that are no multiple of 16 bytes are copied to padded rows first: F with zero weights, whose h, da and du are zero.
  */
 #include "common.cuh"
 #include "operands.cuh"
 #include "gate.cuh"
+#include "gemm_pair.cuh"
+#include "gemm_fp32.cuh"
 
 #include <algorithm>
 
@@ -48,10 +55,6 @@ namespace mb200
 		{
 			return static_cast<int>(std::max<long long>(1, std::min<long long>((elements + 255) / 256, static_cast<long long>(get(ctx)->sm_count) * 8)));
 		}
-		mlTensor_t matrix(const void *data, mlDataType_t dtype, long long rows, int columns)
-		{
-			return make_tensor(data, dtype, make_shape( { static_cast<int>(rows), columns }));
-		}
 
 		struct Problem
 		{
@@ -59,51 +62,165 @@ namespace mb200
 				long long tokens;
 				int embed, hidden, gate;
 		};
-		/* What a run needs of the workspace, and where it lies. */
-		struct Scratch
+		/* Pitches that TMA can address, and what a run needs of the workspace. */
+		struct Plan
 		{
-				float *au = nullptr; // pre-activations, when the caller keeps none
-				float *dh = nullptr;
-				void *h = nullptr, *dau = nullptr;
+				int embed, hidden; // padded
+				bool pack_x, pack_w1, pack_w2;
+				bool keeps; // what the forward pass leaves in `saved` is used: its rows can be addressed
+				void *x = nullptr, *w1 = nullptr, *w2 = nullptr, *dy = nullptr, *h = nullptr, *dau = nullptr;
+				float *au = nullptr, *dh = nullptr, *partials = nullptr;
 				size_t bytes = 0;
-				Scratch(const Problem &p, void *workspace, bool backward, bool own_au)
+				Plan(mlContext_t ctx, const Problem &p, void *workspace, bool backward, bool saved)
 				{
 					Carver carve(workspace);
-					const size_t es = size_of(p.dtype), th = static_cast<size_t>(p.tokens) * p.hidden;
+					const int es = size_of(p.dtype), unit = 16 / es;
+					const int tokens = static_cast<int>(p.tokens);
+					embed = round_up(p.embed, unit);
+					hidden = round_up(p.hidden, unit);
+					pack_x = embed != p.embed;
+					pack_w1 = pack_x || hidden != p.hidden;
+					pack_w2 = hidden != p.hidden;
+					keeps = saved && hidden == p.hidden;
+					const size_t th = static_cast<size_t>(p.tokens) * hidden, te = static_cast<size_t>(p.tokens) * embed;
+					if (pack_x)
+						x = carve.take<uint8_t>(te * es);
+					if (pack_w1)
+						w1 = carve.take<uint8_t>(static_cast<size_t>(2) * hidden * embed * es);
+					if (pack_w2)
+						w2 = carve.take<uint8_t>(static_cast<size_t>(p.embed) * hidden * es);
 					h = carve.take<uint8_t>(th * es);
-					if (own_au)
+					if (!keeps && (backward || p.dtype == DTYPE_FLOAT32))
 						au = carve.take<float>(2 * th);
+					size_t partial = p.dtype == DTYPE_FLOAT16 ? pair_partial_elements(ctx, tokens, p.embed, hidden) : 0; // y
 					if (backward)
 					{
+						if (pack_x)
+							dy = carve.take<uint8_t>(te * es);
 						dau = carve.take<uint8_t>(2 * th * es);
-						dh = carve.take<float>(th);
+						if (p.dtype == DTYPE_FLOAT32)
+							dh = carve.take<float>(th);
+						else
+							partial = std::max( { partial, pair_partial_elements(ctx, tokens, p.embed, 2 * hidden), pair_partial_elements(ctx, 2 * p.hidden, p.embed, tokens),
+									pair_partial_elements(ctx, p.hidden, p.embed, tokens), pair_partial_elements(ctx, p.embed, p.hidden, tokens) });
 					}
+					partials = carve.take<float>(partial);
 					bytes = carve.used;
 				}
 		};
 
+		/* One pass over operands that TMA can address, in either type. */
 		template<typename T>
-		void gate_forward(mlContext_t ctx, const Problem &p, void *h, const float *au)
+		struct Run
 		{
-			const long long n = p.tokens * p.hidden;
-			with_gate(p.gate, [&](auto gate)
-			{
-				kernel_gate<T, decltype(gate)::value> <<<elementwise_blocks(ctx, n), 256, 0, use_stream(ctx)>>>(reinterpret_cast<T*>(h), au, p.tokens, p.hidden);
-			});
-			MB200_COUNT_LAUNCH();
-			check_cuda(ctx, cudaGetLastError(), "gated feed-forward: gate");
+				mlContext_t ctx;
+				const Problem &p;
+				const Plan &plan;
+				const T *x, *w1, *w2, *dy;
+				int tokens;
+				Run(mlContext_t context, const Problem &problem, const Plan &scratch, const mlTensor_t &x_, const mlTensor_t &w1_, const mlTensor_t &w2_, const mlTensor_t &dy_) :
+						ctx(context),
+						p(problem),
+						plan(scratch),
+						x(padded(x_, plan.x, plan.embed, p.tokens, p.tokens, p.embed, 1)),
+						w1(padded(w1_, plan.w1, plan.embed, plan.hidden, p.hidden, p.embed, 2)),
+						w2(padded(w2_, plan.w2, plan.hidden, p.embed, p.embed, p.hidden, 1)),
+						dy(is_empty_descriptor(dy_) ? nullptr : padded(dy_, plan.dy, plan.embed, p.tokens, p.tokens, p.embed, 1)),
+						tokens(static_cast<int>(p.tokens))
+				{
+				}
+				const T* padded(const mlTensor_t &t, void *copy, int pitch, long long padded_rows, long long rows, int columns, int blocks)
+				{
+					if (copy == nullptr)
+						return reinterpret_cast<const T*>(t.data);
+					pack_rows<T>(ctx, reinterpret_cast<T*>(copy), pitch, padded_rows, reinterpret_cast<const T*>(t.data), rows, columns, blocks);
+					return reinterpret_cast<const T*>(copy);
+				}
+				/* d [M, N] = a b^T + beta d */
+				bool product(int M, int N, int K, const T *a, int lda, bool a_mn, const T *b, int ldb, bool b_mn, T *d, int ldd, float beta)
+				{
+					if constexpr (sizeof(T) == 2)
+						return pair_product(ctx, M, N, K, PairOperand { a, lda, a_mn }, PairOperand { b, ldb, b_mn }, PairResult { d, ldd, 1.0f, beta }, plan.partials);
+					else
+						return float_product(ctx, M, N, K, FloatOperand { a, lda, a_mn }, FloatOperand { b, ldb, b_mn }, d, ldd, 1.0f, beta);
+				}
+				/* h, and a and u unless au is null (fp32 needs them) */
+				bool gate(float *au)
+				{
+					if constexpr (sizeof(T) == 2)
+						return pair_gated(ctx, tokens, p.embed, plan.hidden, PairOperand { x, plan.embed, false }, PairOperand { w1, plan.embed, false }, p.gate,
+								reinterpret_cast<__half*>(plan.h), plan.hidden, au);
+					else
+					{
+						if (!product(tokens, 2 * plan.hidden, p.embed, x, plan.embed, false, w1, plan.embed, false, au, 2 * plan.hidden, 0.0f))
+							return false;
+						with_gate(p.gate, [&](auto gate)
+						{
+							kernel_gate<T, decltype(gate)::value> <<<elementwise_blocks(ctx, p.tokens * plan.hidden), 256, 0, use_stream(ctx)>>>(reinterpret_cast<T*>(plan.h), au,
+									p.tokens, plan.hidden);
+						});
+						MB200_COUNT_LAUNCH();
+						return check_cuda(ctx, cudaGetLastError(), "gated feed-forward: gate");
+					}
+				}
+				bool gate_backward(const float *au)
+				{
+					if constexpr (sizeof(T) == 2)
+						return pair_gated_backward(ctx, tokens, p.embed, plan.hidden, PairOperand { dy, plan.embed, false }, PairOperand { w2, plan.hidden, true }, p.gate, au,
+								reinterpret_cast<__half*>(plan.dau), reinterpret_cast<__half*>(plan.h));
+					else
+					{
+						if (!product(tokens, plan.hidden, p.embed, dy, plan.embed, false, w2, plan.hidden, true, plan.dh, plan.hidden, 0.0f))
+							return false;
+						with_gate(p.gate, [&](auto gate)
+						{
+							kernel_gate_backward<T, decltype(gate)::value> <<<elementwise_blocks(ctx, p.tokens * plan.hidden), 256, 0, use_stream(ctx)>>>(
+									reinterpret_cast<T*>(plan.dau), reinterpret_cast<T*>(plan.h), plan.dh, au, p.tokens, plan.hidden);
+						});
+						MB200_COUNT_LAUNCH();
+						return check_cuda(ctx, cudaGetLastError(), "gated feed-forward: gate backward");
+					}
+				}
+				void forward(T *y, float beta, float *saved)
+				{
+					float *au = plan.keeps ? saved : plan.au;
+					const T *h = reinterpret_cast<const T*>(plan.h);
+					if (gate(au))
+						product(tokens, p.embed, plan.hidden, h, plan.hidden, false, w2, plan.hidden, false, y, p.embed, beta);
+				}
+				void backward(const float *saved, float beta_dx, T *dx, float beta_dw, T *dw1, T *dw2)
+				{
+					const float *au = plan.keeps ? saved : plan.au;
+					if ((!plan.keeps && !gate(plan.au)) || !gate_backward(au))
+						return;
+					const T *dau = reinterpret_cast<const T*>(plan.dau), *h = reinterpret_cast<const T*>(plan.h);
+					const int F = plan.hidden;
+					if (dx != nullptr && !product(tokens, p.embed, 2 * F, dau, 2 * F, false, w1, plan.embed, true, dx, p.embed, beta_dx))
+						return;
+					if (dw1 != nullptr)
+					{ // one product, or two where padding separates the gate rows from the up rows
+						const int parts = F == p.hidden ? 1 : 2;
+						for (int i = 0; i < parts; i++)
+							if (!product(2 * p.hidden / parts, p.embed, tokens, dau + i * F, 2 * F, true, x, plan.embed, true, dw1 + static_cast<size_t>(i) * p.hidden * p.embed, p.embed,
+									beta_dw))
+								return;
+					}
+					if (dw2 != nullptr)
+						product(p.embed, p.hidden, tokens, dy, plan.embed, true, h, F, true, dw2, p.hidden, beta_dw);
+				}
+		};
+		/* TMA reads operands whose rows need no padding from where they lie. */
+		bool check_alignment(mlContext_t ctx, const char *who, const char *name, const mlTensor_t &t, bool copied)
+		{
+			if (copied || t.data == nullptr || aligned_to(t.data, 16))
+				return true;
+			record_error(ctx, "%s: %s must be 16-byte aligned", who, name);
+			return false;
 		}
 		template<typename T>
-		void gate_backward(mlContext_t ctx, const Problem &p, const Scratch &s, const float *au)
+		T* data_of(const mlTensor_t &t)
 		{
-			const long long n = p.tokens * p.hidden;
-			with_gate(p.gate, [&](auto gate)
-			{
-				kernel_gate_backward<T, decltype(gate)::value> <<<elementwise_blocks(ctx, n), 256, 0, use_stream(ctx)>>>(reinterpret_cast<T*>(s.dau), reinterpret_cast<T*>(s.h), s.dh,
-						au, p.tokens, p.hidden);
-			});
-			MB200_COUNT_LAUNCH();
-			check_cuda(ctx, cudaGetLastError(), "gated feed-forward: gate backward");
+			return reinterpret_cast<T*>(t.data);
 		}
 
 		bool check_problem(mlContext_t ctx, const char *who, const mlTensor_t &x, const mlTensor_t &w1, const mlTensor_t &w2, int gate, Problem &p)
@@ -130,7 +247,7 @@ namespace mb200
 			p.hidden = w1.dim[0] / 2;
 			p.gate = gate;
 			p.tokens = volume(x) / p.embed;
-			if (p.tokens > 0x7FFFFFFFll / 2)
+			if (p.tokens > 0x3FFFFFFF)
 			{
 				record_error(ctx, "%s: %lld tokens are too many for one call", who, p.tokens);
 				return false;
@@ -150,9 +267,9 @@ extern "C"
 		if (context == nullptr || x_shape.rank < 1 || x_shape.rank > 6 || w1_shape.rank != 2 || w1_shape.dim[0] <= 0 || w1_shape.dim[1] <= 0 || last_dim(x_shape) != w1_shape.dim[1])
 			return 0;
 		const Problem p { dtype, volume_without_last_dim(x_shape), w1_shape.dim[1], w1_shape.dim[0] / 2, MB200_GATE_SILU };
-		if (p.tokens <= 0)
+		if (p.tokens <= 0 || p.tokens > 0x3FFFFFFF || (dtype != DTYPE_FLOAT16 && dtype != DTYPE_FLOAT32))
 			return 0;
-		return Scratch(p, nullptr, training, !saved).bytes;
+		return std::max(Plan(context, p, nullptr, false, training && saved).bytes, training ? Plan(context, p, nullptr, true, saved).bytes : 0);
 	}
 
 	void mb200_gated_feed_forward_forward(mlContext_t context, const mlTensor_t x, const mlTensor_t w1, const mlTensor_t w2, float beta, mlTensor_t y, int gate, mlTensor_t saved,
@@ -168,8 +285,9 @@ extern "C"
 			return;
 		if (p.tokens == 0)
 			return;
-		const Scratch need(p, nullptr, false, !keep);
-		if (!check_workspace(context, who, workspace, need.bytes))
+		const Plan plan(context, p, workspace.data, false, keep);
+		if (!check_workspace(context, who, workspace, plan.bytes) || !check_alignment(context, who, "x", x, plan.pack_x) || !check_alignment(context, who, "w1", w1, plan.pack_w1)
+				|| !check_alignment(context, who, "w2", w2, plan.pack_w2) || !check_alignment(context, who, "saved", saved, !plan.keeps))
 			return;
 		const struct { const char *name; const mlTensor_t &t; } inputs[] = { { "x", x }, { "w1", w1 }, { "w2", w2 } }, results[] = { { "y", y }, { "saved", saved }, { "workspace", workspace } };
 		for (int i = 0; i < 3; i++)
@@ -182,15 +300,10 @@ extern "C"
 					return;
 		}
 		flush_pending(context);
-		const Scratch s(p, workspace.data, false, !keep);
-		float *au = keep ? reinterpret_cast<float*>(saved.data) : s.au;
-		const mlTensor_t x2 = matrix(x.data, p.dtype, p.tokens, p.embed);
-		cuda_gemm_v2(context, 'n', 't', 1.0f, x2, w1, 0.0f, matrix(au, DTYPE_FLOAT32, p.tokens, 2 * p.hidden));
 		if (p.dtype == DTYPE_FLOAT16)
-			gate_forward<__half>(context, p, s.h, au);
+			Run<__half>(context, p, plan, x, w1, w2, no_tensor()).forward(data_of<__half>(y), beta, data_of<float>(saved));
 		else
-			gate_forward<float>(context, p, s.h, au);
-		cuda_gemm_v2(context, 'n', 't', 1.0f, matrix(s.h, p.dtype, p.tokens, p.hidden), w2, beta, matrix(y.data, p.dtype, p.tokens, p.embed));
+			Run<float>(context, p, plan, x, w1, w2, no_tensor()).forward(data_of<float>(y), beta, data_of<float>(saved));
 	}
 
 	void mb200_gated_feed_forward_backward(mlContext_t context, const mlTensor_t x, const mlTensor_t w1, const mlTensor_t w2, const mlTensor_t saved, const mlTensor_t dy, float beta_dx,
@@ -207,8 +320,18 @@ extern "C"
 				|| (want_dw1 && !check_operand(context, who, "dw1", dw1, x.dtype, 2ll * p.hidden, p.embed))
 				|| (want_dw2 && !check_operand(context, who, "dw2", dw2, x.dtype, p.embed, p.hidden)))
 			return;
-		const Scratch need(p, nullptr, true, !kept);
-		if (p.tokens > 0 && !check_workspace(context, who, workspace, need.bytes))
+		if (p.tokens == 0)
+		{ // no tokens: the weight gradients are sums of nothing
+			if (want_dw1)
+				cuda_scale_tensor(context, beta_dw, dw1);
+			if (want_dw2)
+				cuda_scale_tensor(context, beta_dw, dw2);
+			return;
+		}
+		const Plan plan(context, p, workspace.data, true, kept);
+		if (!check_workspace(context, who, workspace, plan.bytes) || !check_alignment(context, who, "x", x, plan.pack_x) || !check_alignment(context, who, "dy", dy, plan.pack_x)
+				|| !check_alignment(context, who, "w1", w1, plan.pack_w1) || !check_alignment(context, who, "w2", w2, plan.pack_w2)
+				|| !check_alignment(context, who, "saved", saved, !plan.keeps))
 			return;
 		const struct { const char *name; const mlTensor_t &t; } inputs[] = { { "x", x }, { "w1", w1 }, { "w2", w2 }, { "saved", saved }, { "dy", dy } }, results[] = { { "dx", dx },
 				{ "dw1", dw1 }, { "dw2", dw2 }, { "workspace", workspace } };
@@ -222,30 +345,9 @@ extern "C"
 					return;
 		}
 		flush_pending(context);
-		if (p.tokens == 0)
-		{ // no tokens: the weight gradients are sums of nothing
-			if (want_dw1)
-				cuda_scale_tensor(context, beta_dw, dw1);
-			if (want_dw2)
-				cuda_scale_tensor(context, beta_dw, dw2);
-			return;
-		}
-		const Scratch s(p, workspace.data, true, !kept);
-		const float *au = kept ? reinterpret_cast<const float*>(saved.data) : s.au;
-		const mlTensor_t x2 = matrix(x.data, p.dtype, p.tokens, p.embed), dy2 = matrix(dy.data, p.dtype, p.tokens, p.embed);
-		if (!kept)
-			cuda_gemm_v2(context, 'n', 't', 1.0f, x2, w1, 0.0f, matrix(au, DTYPE_FLOAT32, p.tokens, 2 * p.hidden));
-		cuda_gemm_v2(context, 'n', 'n', 1.0f, dy2, w2, 0.0f, matrix(s.dh, DTYPE_FLOAT32, p.tokens, p.hidden));
 		if (p.dtype == DTYPE_FLOAT16)
-			gate_backward<__half>(context, p, s, au);
+			Run<__half>(context, p, plan, x, w1, w2, dy).backward(data_of<float>(saved), beta_dx, data_of<__half>(dx), beta_dw, data_of<__half>(dw1), data_of<__half>(dw2));
 		else
-			gate_backward<float>(context, p, s, au);
-		const mlTensor_t dau = matrix(s.dau, p.dtype, p.tokens, 2 * p.hidden);
-		if (want_dx)
-			cuda_gemm_v2(context, 'n', 'n', 1.0f, dau, w1, beta_dx, matrix(dx.data, p.dtype, p.tokens, p.embed));
-		if (want_dw1)
-			cuda_gemm_v2(context, 't', 'n', 1.0f, dau, x2, beta_dw, dw1);
-		if (want_dw2)
-			cuda_gemm_v2(context, 't', 'n', 1.0f, dy2, matrix(s.h, p.dtype, p.tokens, p.hidden), beta_dw, dw2);
+			Run<float>(context, p, plan, x, w1, w2, dy).backward(data_of<float>(saved), beta_dx, data_of<float>(dx), beta_dw, data_of<float>(dw1), data_of<float>(dw2));
 	}
 }

@@ -125,6 +125,15 @@ namespace mb200
 				return result;
 			}
 	};
+	inline int round_up(int n, int to)
+	{
+		return (n + to - 1) / to * to;
+	}
+	inline mlTensor_t no_tensor()
+	{
+		mlTensor_t t = { };
+		return t;
+	}
 	/* Launch whose grid may start before the grid ahead of it in the stream has finished; the kernel calls griddepcontrol.wait
 	 * (wait_for_previous_grid) before it touches anything that grid wrote. */
 	template<typename ... KArgs, typename ... Args>
