@@ -197,7 +197,7 @@ namespace mb200
 				int piece, pitch; // columns of a piece of logits or probabilities, and its rows' pitch
 				int dx_splits; // fp32 sums that dx is kept in until the last piece
 				float2 *running = nullptr; // fp32: per row; fp16: per row and 128 columns
-				float *target_logit = nullptr, *z = nullptr, *dx_sums = nullptr, *partials = nullptr, *largest = nullptr;
+				float *target_logit = nullptr, *z = nullptr, *dx_sums = nullptr, *dw_sum = nullptr, *partials = nullptr, *largest = nullptr;
 				void *p = nullptr, *x = nullptr, *w = nullptr, *weighted_x = nullptr;
 				size_t bytes = 0;
 				Plan(mlContext_t ctx, const Problem &q, void *workspace, bool training, int columns)
@@ -228,11 +228,21 @@ namespace mb200
 						weighted_x = carve.take<uint8_t>(rows * es);
 						p = half ? carve.take<uint8_t>(cells * es) : nullptr; // fp32: in place of the logits
 						dx_sums = carve.take<float>(rows * dx_splits);
-						// dW of a piece: fp16 may be cut along K, fp32 goes through a sum so that a device-side factor can be applied
-						const int last = q.vocab - (q.vocab - 1) / piece * piece;
-						partials = carve.take<float>(half ? std::max(pair_partial_elements(ctx, piece, q.embed, tokens), pair_partial_elements(ctx, last, q.embed, tokens))
-								: static_cast<size_t>(piece) * embed);
+						if (!half) // dW of a piece, to which a factor that only the device knows is applied
+							dw_sum = carve.take<float>(static_cast<size_t>(piece) * embed);
 					}
+					// products that are cut along K: of a whole piece, and of the last, narrower one
+					size_t partial = 0;
+					for (int width : { piece, q.vocab - (q.vocab - 1) / piece * piece })
+					{
+						if (half && training)
+							partial = std::max(partial, pair_partial_elements(ctx, width, q.embed, tokens));
+						if (!half)
+							partial = std::max(partial, float_partial_elements(ctx, tokens, width, q.embed));
+						if (!half && training)
+							partial = std::max( { partial, float_partial_elements(ctx, tokens, q.embed, width), float_partial_elements(ctx, width, q.embed, tokens) });
+					}
+					partials = carve.take<float>(partial);
 					bytes = carve.used;
 				}
 		};
@@ -340,7 +350,7 @@ namespace mb200
 			{
 				const int width = std::min(plan.piece, q.vocab - first);
 				if (!float_product(ctx, static_cast<int>(q.tokens), width, q.embed, FloatOperand { o.x, plan.embed, false },
-						FloatOperand { o.w + static_cast<size_t>(first) * plan.embed, plan.embed, false }, plan.z, plan.pitch, 1.0f, 0.0f))
+						FloatOperand { o.w + static_cast<size_t>(first) * plan.embed, plan.embed, false }, plan.z, plan.pitch, 0.0f, plan.partials))
 					return;
 				kernel_piece_statistics<<<row_blocks(ctx, q.tokens), 256, 0, use_stream(ctx)>>>(plan.z, plan.pitch, plan.running, plan.target_logit, rows, q.tokens, first, width,
 						first + width == q.vocab, loss, lse);
@@ -388,18 +398,18 @@ namespace mb200
 				}
 				else
 				{
-					if (!float_product(ctx, tokens, width, D, FloatOperand { o.x, ld, false }, FloatOperand { w, ld, false }, plan.z, plan.pitch, 1.0f, 0.0f))
+					if (!float_product(ctx, tokens, width, D, FloatOperand { o.x, ld, false }, FloatOperand { w, ld, false }, plan.z, plan.pitch, 0.0f, plan.partials))
 						return;
 					kernel_piece_gradient<<<elementwise_blocks(ctx, q.tokens * width), 256, 0, stream>>>(plan.z, plan.pitch, lse, rows, q.tokens, first, width);
 					MB200_COUNT_LAUNCH();
 					if (!check_cuda(ctx, cudaGetLastError(), "mb200_softmax_cross_entropy_backward: probabilities"))
 						return;
 					if (dx != nullptr
-							&& !float_product(ctx, tokens, D, width, FloatOperand { plan.z, plan.pitch, false }, FloatOperand { w, ld, true }, plan.dx_sums, ld, 1.0f, first > 0 ? 1.0f : 0.0f))
+							&& !float_product(ctx, tokens, D, width, FloatOperand { plan.z, plan.pitch, false }, FloatOperand { w, ld, true }, plan.dx_sums, ld, first > 0 ? 1.0f : 0.0f, plan.partials))
 						return;
 					if (dw != nullptr
-							&& (!float_product(ctx, width, D, tokens, FloatOperand { plan.z, plan.pitch, true }, FloatOperand { weighted_x, ld, true }, plan.partials, ld, 1.0f, 0.0f)
-									|| !finish_sums<float>(ctx, dw + static_cast<size_t>(first) * D, D, width, D, plan.partials, ld, 1, unscale, largest, nullptr, beta_dw)))
+							&& (!float_product(ctx, width, D, tokens, FloatOperand { plan.z, plan.pitch, true }, FloatOperand { weighted_x, ld, true }, plan.dw_sum, ld, 0.0f, plan.partials)
+									|| !finish_sums<float>(ctx, dw + static_cast<size_t>(first) * D, D, width, D, plan.dw_sum, ld, 1, unscale, largest, nullptr, beta_dw)))
 						return;
 				}
 			}

@@ -92,17 +92,24 @@ namespace mb200
 					h = carve.take<uint8_t>(th * es);
 					if (!keeps && (backward || p.dtype == DTYPE_FLOAT32))
 						au = carve.take<float>(2 * th);
-					size_t partial = p.dtype == DTYPE_FLOAT16 ? pair_partial_elements(ctx, tokens, p.embed, hidden) : 0; // y
+					auto cut = [&](int M, int N, int K)
+					{
+						return p.dtype == DTYPE_FLOAT16 ? pair_partial_elements(ctx, M, N, K) : float_partial_elements(ctx, M, N, K);
+					};
+					size_t partial = cut(tokens, p.embed, hidden); // y
+					if (p.dtype == DTYPE_FLOAT32)
+						partial = std::max(partial, cut(tokens, 2 * hidden, p.embed));
 					if (backward)
 					{
 						if (pack_x)
 							dy = carve.take<uint8_t>(te * es);
 						dau = carve.take<uint8_t>(2 * th * es);
 						if (p.dtype == DTYPE_FLOAT32)
+						{
 							dh = carve.take<float>(th);
-						else
-							partial = std::max( { partial, pair_partial_elements(ctx, tokens, p.embed, 2 * hidden), pair_partial_elements(ctx, 2 * p.hidden, p.embed, tokens),
-									pair_partial_elements(ctx, p.hidden, p.embed, tokens), pair_partial_elements(ctx, p.embed, p.hidden, tokens) });
+							partial = std::max(partial, cut(tokens, hidden, p.embed));
+						}
+						partial = std::max( { partial, cut(tokens, p.embed, 2 * hidden), cut(2 * p.hidden, p.embed, tokens), cut(p.hidden, p.embed, tokens), cut(p.embed, p.hidden, tokens) });
 					}
 					partials = carve.take<float>(partial);
 					bytes = carve.used;
@@ -142,7 +149,7 @@ namespace mb200
 					if constexpr (sizeof(T) == 2)
 						return pair_product(ctx, M, N, K, PairOperand { a, lda, a_mn }, PairOperand { b, ldb, b_mn }, PairResult { d, ldd, 1.0f, beta }, plan.partials);
 					else
-						return float_product(ctx, M, N, K, FloatOperand { a, lda, a_mn }, FloatOperand { b, ldb, b_mn }, d, ldd, 1.0f, beta);
+						return float_product(ctx, M, N, K, FloatOperand { a, lda, a_mn }, FloatOperand { b, ldb, b_mn }, d, ldd, beta, plan.partials);
 				}
 				/* h, and a and u unless au is null (fp32 needs them) */
 				bool gate(float *au)

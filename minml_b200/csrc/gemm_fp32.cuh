@@ -14,8 +14,9 @@ namespace mb200
 			int ld = 0;
 			bool mn = false;
 	};
-	/* D = alpha A B^T + beta D, fp32 */
-	bool float_product(mlContext_t ctx, int M, int N, int K, const FloatOperand &a, const FloatOperand &b, float *d, int ldd, float alpha, float beta);
+	/* D = A B^T + beta D, fp32; `partials` holds float_partial_elements(M, N, K) floats. */
+	size_t float_partial_elements(mlContext_t ctx, int M, int N, int K);
+	bool float_product(mlContext_t ctx, int M, int N, int K, const FloatOperand &a, const FloatOperand &b, float *d, int ldd, float beta, float *partials);
 
 	/* dst [blocks * padded_rows, pitch] = src [blocks * rows, columns], the added rows and columns zero */
 	template<typename T>
