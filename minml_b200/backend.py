@@ -5,6 +5,7 @@ libminml_b200.so through ctypes -- the same calls, in the same argument order, t
 torch is used for device memory only.  After every call the context's sticky error is checked and raised.
 """
 import ctypes
+import struct
 
 import torch
 
@@ -46,22 +47,22 @@ def _check_device(t, ctx):
         raise BackendError("tensor on cuda:%d passed to a context of cuda:%d" % (t.device.index, ctx.device_index))
 
 
+_EMPTY = mlTensor_t()  # null data, rank 0 (passed by value, so one instance serves every absent operand)
+_EMPTY.dtype = _abi.DTYPE_UNKNOWN
+_PACK = struct.Struct("@Qii6i").pack  # the layout of mlTensor_t; packing at once costs half of setting the fields one by one
+_FILL = [(0,) * (6 - i) for i in range(7)]
+
+
 def desc(t, ctx=None):
     """mlTensor_t for a dense torch tensor; None gives the empty descriptor (null data, rank 0)."""
-    d = mlTensor_t()
     if t is None:
-        d.data = None
-        d.dtype = _abi.DTYPE_UNKNOWN
-        d.rank = 0
-        return d
+        return _EMPTY
     assert t.is_contiguous(), "the backend ABI addresses dense row-major tensors only"
-    _check_device(t, ctx)
-    d.data = t.data_ptr()
-    d.dtype = dtype_of(t)
-    d.rank = t.dim()
-    for i, n in enumerate(t.shape):
-        d.dim[i] = int(n)
-    return d
+    if ctx is not None:
+        _check_device(t, ctx)
+    shape = t.shape
+    rank = len(shape)
+    return mlTensor_t.from_buffer_copy(_PACK(t.data_ptr(), _DTYPES[t.dtype], rank, *shape, *_FILL[rank]))
 
 
 def ptr(t, ctx=None):

@@ -13,8 +13,8 @@
  * relative precision down to 2^-29).  Row weights do not go into P, where small ones would cost dx its digits, but into dx's fp32
  * result and into a copy of x, as c_t / max |c| (exact where all weights are equal).
  *
- * fp16 runs on gemm_pair.cu: forward is one product whose epilogue leaves (maximum, sum of exponentials) for every row and 128 columns,
- * joined by a second kernel, and the whole vocabulary is one piece; backward makes 2^15 P of a piece in the epilogue of its logits and
+ * fp16 runs on gemm_pair.cu (up to 64 rows forward: few_tokens.cu): forward is one product whose epilogue leaves (maximum, sum of
+ * exponentials) for every row and group of columns, joined by a second kernel, and the whole vocabulary is one piece; backward makes 2^15 P of a piece in the epilogue of its logits and
  * multiplies it with W and x.  dx is added up over the pieces in fp32.  fp32 keeps one piece's logits.  An embed that is no multiple of 16
  * bytes is copied to padded rows first.
  */
@@ -22,6 +22,7 @@
 #include "operands.cuh"
 #include "gemm_pair.cuh"
 #include "gemm_fp32.cuh"
+#include "few_tokens.cuh"
 
 #include <algorithm>
 
@@ -161,24 +162,28 @@ namespace mb200
 					out[t * embed + k] = factor == 0.0f ? from_float<T>(0.0f) : from_float<T>(to_float(x[t * embed + k]) * factor);
 			}
 		}
-		/* Joins the groups' statistics of a row: a block takes 32 rows, its 32 warps every 32nd group. */
-		__global__ void __launch_bounds__(1024) kernel_join_statistics(const float2 *__restrict__ parts, int groups, const float *__restrict__ target_logit, Rows rows, long long tokens,
+		/* Joins the statistics of a row's groups, parts[t][group]: a block a row. */
+		__global__ void __launch_bounds__(256) kernel_join_statistics(const float2 *__restrict__ parts, int groups, const float *__restrict__ target_logit, Rows rows,
 				float *__restrict__ loss, float *__restrict__ lse)
 		{
-			__shared__ float2 scratch[32][33];
-			const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-			const long long t = static_cast<long long>(blockIdx.x) * 32 + lane;
+			__shared__ float2 scratch[8];
+			const long long t = blockIdx.x;
 			wait_for_previous_grid();
 			float2 mine = make_float2(-INFINITY, 0.0f);
-			if (t < tokens)
-				for (int g = warp; g < groups; g += 32)
-					mine = merge(mine, parts[g * tokens + t]);
-			scratch[lane][warp] = mine;
+#pragma unroll 4
+			for (int g = threadIdx.x; g < groups; g += 256)
+				mine = merge(mine, parts[t * groups + g]);
+			mine = merge_warp(mine);
+			if (threadIdx.x % 32 == 0)
+				scratch[threadIdx.x / 32] = mine;
 			__syncthreads();
-			const float2 total = merge_warp(scratch[warp][lane]);
-			const long long row = static_cast<long long>(blockIdx.x) * 32 + warp;
-			if (lane == 0 && row < tokens)
-				finish_row(row, total, rows, target_logit, loss, lse);
+			if (threadIdx.x == 0)
+			{
+				float2 total = scratch[0];
+				for (int k = 1; k < 8; k++)
+					total = merge(total, scratch[k]);
+				finish_row(t, total, rows, target_logit, loss, lse);
+			}
 		}
 
 		int elementwise_blocks(mlContext_t ctx, long long elements)
@@ -190,6 +195,10 @@ namespace mb200
 			return static_cast<int>(std::max<long long>(1, std::min<long long>(rows, static_cast<long long>(get(ctx)->sm_count) * 8)));
 		}
 
+		int statistics_groups(mlContext_t ctx, const Problem &q)
+		{
+			return q.tokens <= FEW_TOKENS ? few_statistics_parts(ctx, q.vocab) : pair_statistics_parts(q.vocab);
+		}
 		/* The workspace of one call with pieces of `piece` columns. */
 		struct Plan
 		{
@@ -218,7 +227,7 @@ namespace mb200
 					if (!training)
 					{
 						target_logit = carve.take<float>(q.tokens);
-						running = carve.take<float2>(q.tokens * (half ? pair_statistics_parts(q.vocab) : 1));
+						running = carve.take<float2>(q.tokens * (half ? statistics_groups(ctx, q) : 1));
 					}
 					if (!half)
 						z = carve.take<float>(cells);
@@ -336,11 +345,15 @@ namespace mb200
 
 		void forward_half(mlContext_t ctx, const Problem &q, const Rows &rows, const Plan &plan, const Operands<__half> &o, float *loss, float *lse)
 		{
-			if (!pair_statistics(ctx, static_cast<int>(q.tokens), q.vocab, q.embed, PairOperand { o.x, plan.embed, false }, PairOperand { o.w, plan.embed, false }, rows.targets,
-					plan.running, plan.target_logit))
+			const int tokens = static_cast<int>(q.tokens);
+			const bool ok = tokens <= FEW_TOKENS
+					? few_statistics(ctx, FewTokens { tokens, plan.embed, o.x, plan.embed, o.w, plan.embed }, q.vocab, rows.targets, plan.running, plan.target_logit)
+					: pair_statistics(ctx, tokens, q.vocab, q.embed, PairOperand { o.x, plan.embed, false }, PairOperand { o.w, plan.embed, false }, rows.targets, plan.running,
+							plan.target_logit);
+			if (!ok)
 				return;
-			const cudaError_t status = launch_overlapped(kernel_join_statistics, dim3(static_cast<unsigned>((q.tokens + 31) / 32)), dim3(1024), 0, use_stream(ctx), plan.running,
-					pair_statistics_parts(q.vocab), plan.target_logit, rows, q.tokens, loss, lse);
+			const cudaError_t status = launch_overlapped(kernel_join_statistics, dim3(tokens), dim3(256), 0, use_stream(ctx), plan.running, statistics_groups(ctx, q), plan.target_logit, rows,
+					loss, lse);
 			MB200_COUNT_LAUNCH();
 			check_cuda(ctx, status, "mb200_softmax_cross_entropy_forward");
 		}

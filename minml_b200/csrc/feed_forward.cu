@@ -16,6 +16,7 @@
 #include "gate.cuh"
 #include "gemm_pair.cuh"
 #include "gemm_fp32.cuh"
+#include "few_tokens.cuh"
 
 #include <algorithm>
 
@@ -192,6 +193,13 @@ namespace mb200
 				{
 					float *au = plan.keeps ? saved : plan.au;
 					const T *h = reinterpret_cast<const T*>(plan.h);
+					if constexpr (sizeof(T) == 2)
+						if (tokens <= FEW_TOKENS && au == nullptr)
+						{ // decoding: both launches stream their weights once
+							if (few_gated(ctx, FewTokens { tokens, plan.embed, x, plan.embed, w1, plan.embed }, plan.hidden, p.gate, reinterpret_cast<__half*>(plan.h), plan.hidden))
+								few_product(ctx, FewTokens { tokens, plan.hidden, h, plan.hidden, w2, plan.hidden }, p.embed, y, p.embed, beta, true);
+							return;
+						}
 					if (gate(au))
 						product(tokens, p.embed, plan.hidden, h, plan.hidden, false, w2, plan.hidden, false, y, p.embed, beta);
 				}

@@ -74,6 +74,7 @@ namespace mb200
 				const float *row_weights, *lse;
 				int first, vocab;
 				float2 *parts;
+				int groups;
 				float *target_logit;
 				int *status;
 		};
@@ -362,7 +363,7 @@ namespace mb200
 							sum += j < valid ? exp2_approx(fmaf(v[j], LOG2E, -shift)) : 0.0f;
 						if (row_ok && valid > 0)
 						{
-							p.parts[static_cast<long long>(u.nt * 2 + half) * p.M + row] = make_float2(top, sum);
+							p.parts[static_cast<long long>(row) * p.groups + u.nt * 2 + half] = make_float2(top, sum);
 							if (at >= 0 && at < min(BN / 2, valid))
 								p.target_logit[row] = target;
 						}
@@ -894,6 +895,7 @@ namespace mb200
 			return false;
 		p.targets = targets;
 		p.parts = parts;
+		p.groups = pair_statistics_parts(N);
 		p.target_logit = target_logit;
 		return launch<STATISTICS, 0>(ctx, maps, p);
 	}

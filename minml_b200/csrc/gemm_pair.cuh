@@ -45,7 +45,7 @@ namespace mb200
 	 * multiple of 8. */
 	bool pair_gated_backward(mlContext_t ctx, int tokens, int embed, int hidden, const PairOperand &dy, const PairOperand &w2, int gate, const float *au, __half *dau, __half *h);
 
-	/* Row statistics of the logits x w^T over columns first .. first + N: parts[i][t] = (maximum, sum of exp(z - maximum)) of a group of
+	/* Row statistics of the logits x w^T over columns first .. first + N: parts[t][i] = (maximum, sum of exp(z - maximum)) of group i of
 	 * 128 columns, pair_statistics_parts(N) groups; target_logit[t] where the row's target lies in the range. */
 	int pair_statistics_parts(int N);
 	bool pair_statistics(mlContext_t ctx, int tokens, int N, int embed, const PairOperand &x, const PairOperand &w, const int *targets, float2 *parts, float *target_logit);
