@@ -53,7 +53,8 @@ namespace mb200
 			STORE, // fp16 result
 			SUMS, // fp32 sums, stored or added
 			GATED,
-			GATED_BACKWARD,
+			GATED_BACKWARD, // from a kept a and u
+			GATED_RECOMPUTE, // the same, with a and u made again in the same tile
 			STATISTICS,
 			PROBABILITIES
 		};
@@ -82,6 +83,7 @@ namespace mb200
 		{
 				uint64_t full[STAGES], empty[STAGES];
 				uint64_t tmem_full[2], tmem_empty[2];
+				uint64_t au_empty; // GATED_RECOMPUTE: a and u have been read
 				uint32_t tmem_base;
 				int abort_flag;
 		};
@@ -131,7 +133,8 @@ namespace mb200
 		}
 		template<int EPI, int GATE>
 		__global__ void __launch_bounds__(THREADS, 1) kernel_gemm_pair(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-				const __grid_constant__ CUtensorMap map_d, const __grid_constant__ CUtensorMap map_e, const __grid_constant__ CUtensorMap map_f, const Params p)
+				const __grid_constant__ CUtensorMap map_d, const __grid_constant__ CUtensorMap map_e, const __grid_constant__ CUtensorMap map_f,
+				const __grid_constant__ CUtensorMap map_dy, const __grid_constant__ CUtensorMap map_w2, const Params p)
 		{
 			extern __shared__ uint8_t smem_raw[];
 			__shared__ Barriers bars;
@@ -176,6 +179,7 @@ namespace mb200
 					mbar_init(smem_u32(&bars.tmem_full[a]), 1);
 					mbar_init(smem_u32(&bars.tmem_empty[a]), 2 * EPI_WARPS);
 				}
+				mbar_init(smem_u32(&bars.au_empty), 2 * EPI_WARPS);
 				bars.abort_flag = 0;
 				fence_mbar_init();
 			}
@@ -203,8 +207,24 @@ namespace mb200
 					for (int unit = first_unit; unit < units && ok; unit += unit_step)
 					{
 						const Unit u = locate(unit);
-						const int n0 = EPI == GATED ? u.nt * (BN / 2) + (leader ? 0 : p.up_row) : u.nt * BN + static_cast<int>(rank) * (BN / 2);
-						for (int kb = u.kb0; kb < u.kb1; kb++, it++)
+						const int n0 = EPI == GATED || EPI == GATED_RECOMPUTE ? u.nt * (BN / 2) + (leader ? 0 : p.up_row) : u.nt * BN + static_cast<int>(rank) * (BN / 2);
+						if (EPI == GATED_RECOMPUTE)
+							for (int kb = u.kb0; kb < u.kb1 && ok; kb++, it++)
+							{ // dy and 64 columns of W2
+								const int s = it % STAGES;
+								if (!mbar_wait(smem_u32(&bars.empty[s]), ((it / STAGES) & 1u) ^ 1u, abort_flag))
+								{
+									ok = false;
+									break;
+								}
+								const uint32_t full = smem_u32(&bars.full[s]);
+								if (leader)
+									mbar_arrive_expect_tx(full, 2 * (OPERAND_BYTES + OPERAND_BYTES / 2));
+								const uint32_t full_leader = map_to_cta(full, 0);
+								tma_load_2d_pair(smem_base + s * STAGE_BYTES, &map_dy, full_leader, kb * BK, u.m0);
+								tma_load_2d_pair(smem_base + s * STAGE_BYTES + OPERAND_BYTES, &map_w2, full_leader, u.nt * (BN / 2) + static_cast<int>(rank) * 64, kb * BK);
+							}
+						for (int kb = u.kb0; kb < u.kb1 && ok; kb++, it++)
 						{
 							const int s = it % STAGES;
 							if (!mbar_wait(smem_u32(&bars.empty[s]), ((it / STAGES) & 1u) ^ 1u, abort_flag))
@@ -248,17 +268,47 @@ namespace mb200
 					for (int unit = first_unit; unit < units && ok; unit += unit_step)
 					{
 						const Unit u = locate(unit);
+						if (EPI == GATED_RECOMPUTE)
+						{ // dh into columns 256 + 128 i, two buffers; a and u, below, into columns 0 .. 255
+							const uint32_t acc = buffers & 1u;
+							if (!mbar_wait_cluster(smem_u32(&bars.tmem_empty[acc]), ((buffers >> 1) & 1u) ^ 1u, abort_flag))
+								break;
+							tcgen05_fence_after();
+							const uint32_t idesc_dh = make_idesc_f16_pair(BN / 2) | (1u << 16);
+							for (int kb = u.kb0; kb < u.kb1; kb++, it++)
+							{
+								const int s = it % STAGES;
+								if (!mbar_wait(smem_u32(&bars.full[s]), (it / STAGES) & 1u, abort_flag))
+								{
+									ok = false;
+									break;
+								}
+								tcgen05_fence_after();
+								const uint32_t a = smem_base + s * STAGE_BYTES;
+								const uint64_t desc_a = make_desc_k_sw128(a), desc_b = make_desc_mn_sw128(a + OPERAND_BYTES, OPERAND_BYTES / 2);
+#pragma unroll
+								for (int k = 0; k < 4; k++)
+									mma_ss_pair<0>(tmem_base + BN + acc * (BN / 2), desc_a + 2 * k, desc_b + 128 * k, idesc_dh, kb > u.kb0 || k > 0 ? 1u : 0u);
+								mma_commit_pair(smem_u32(&bars.empty[s]));
+							}
+							if (!ok || !mbar_wait_cluster(smem_u32(&bars.au_empty), (buffers & 1u) ^ 1u, abort_flag))
+								break;
+							tcgen05_fence_after();
+						}
 						for (int kb = u.kb0; kb < u.kb1 && ok;)
 						{ // one accumulator buffer: a whole K range, or a segment of it
 							const int end = min(u.kb1, kb + SEGMENT);
 							const uint32_t acc = buffers & 1u;
-							if (!mbar_wait_cluster(smem_u32(&bars.tmem_empty[acc]), ((buffers >> 1) & 1u) ^ 1u, abort_flag))
+							if (EPI != GATED_RECOMPUTE)
 							{
-								ok = false;
-								break;
+								if (!mbar_wait_cluster(smem_u32(&bars.tmem_empty[acc]), ((buffers >> 1) & 1u) ^ 1u, abort_flag))
+								{
+									ok = false;
+									break;
+								}
+								tcgen05_fence_after();
 							}
-							tcgen05_fence_after();
-							const uint32_t d = tmem_base + acc * BN;
+							const uint32_t d = tmem_base + (EPI == GATED_RECOMPUTE ? 0 : acc * BN);
 							uint32_t accumulate = 0;
 							for (; kb < end; kb++, it++)
 							{
@@ -437,6 +487,61 @@ namespace mb200
 							if (lane == 0 && row0 < p.M)
 							{
 								tma_store_2d(&map_d, box, n, row0);
+								bulk_commit_group();
+							}
+						}
+						continue;
+					}
+
+					if constexpr (EPI == GATED_RECOMPUTE)
+					{
+						// a and u of this warp's 64 hidden columns into registers, so that the next tile's may be made under the arithmetic
+						const int column = half * 64;
+						const uint32_t au = lane_base + column, dh = lane_base + BN + (buffers & 1u) * (BN / 2) + column;
+						uint32_t a[2][32], b[2][32];
+						tmem_ld_32x32(au, a[0]);
+						tmem_ld_32x32(au + BN / 2, b[0]);
+						tmem_ld_32x32(au + 32, a[1]);
+						tmem_ld_32x32(au + BN / 2 + 32, b[1]);
+						tmem_wait_ld();
+						tcgen05_fence_before();
+						__syncwarp();
+						if (lane == 0)
+							mbar_arrive_cluster(map_to_cta(smem_u32(&bars.au_empty), 0));
+#pragma unroll
+						for (int c = 0; c < 2; c++)
+						{
+							const int n = u.nt * (BN / 2) + column + c * 32;
+							float v[32], da[32];
+							load_chunk(dh + c * 32, v);
+							if (c == 1)
+								release();
+							if (n >= p.N)
+								continue; // warp-uniform
+							if (lane == 0)
+								bulk_wait_group_read<0>();
+							__syncwarp();
+#pragma unroll
+							for (int j = 0; j < 32; j++)
+							{
+								float value, derivative;
+								gate_with_derivative<GATE, true>(__uint_as_float(a[c][j]), value, derivative);
+								da[j] = v[j] * __uint_as_float(b[c][j]) * derivative;
+								b[c][j] = __float_as_uint(__uint_as_float(b[c][j]) * value); // h
+								v[j] *= value; // du
+							}
+							write_half_box(staging, lane, da);
+							write_half_box(staging + HALF_BOX, lane, v);
+#pragma unroll
+							for (int j = 0; j < 32; j++)
+								v[j] = __uint_as_float(b[c][j]);
+							write_half_box(staging + 2 * HALF_BOX, lane, v);
+							publish();
+							if (lane == 0 && row0 < p.M)
+							{
+								tma_store_2d(&map_d, staging, n, row0);
+								tma_store_2d(&map_e, staging + HALF_BOX, n, row0);
+								tma_store_2d(&map_f, staging + 2 * HALF_BOX, n, row0);
 								bulk_commit_group();
 							}
 						}
@@ -629,7 +734,7 @@ namespace mb200
 
 		struct Maps
 		{
-				CUtensorMap a, b, d, e, f;
+				CUtensorMap a, b, d, e, f, dy, w2;
 		};
 		template<int EPI, int GATE>
 		bool launch(mlContext_t ctx, const Maps &maps, Params p)
@@ -656,7 +761,7 @@ namespace mb200
 			config.stream = use_stream(ctx);
 			config.attrs = attributes;
 			config.numAttrs = 2;
-			const cudaError_t status = cudaLaunchKernelEx(&config, kernel_gemm_pair<EPI, GATE>, maps.a, maps.b, maps.d, maps.e, maps.f, p);
+			const cudaError_t status = cudaLaunchKernelEx(&config, kernel_gemm_pair<EPI, GATE>, maps.a, maps.b, maps.d, maps.e, maps.f, maps.dy, maps.w2, p);
 			MB200_COUNT_LAUNCH();
 			c->kernels_with_waits = true;
 			return check_cuda(ctx, status, "gemm_pair launch");
@@ -690,7 +795,7 @@ namespace mb200
 			std::memset(&p, 0, sizeof(p));
 			if (!map_operand(ctx, &maps.a, a, M, K) || !map_operand(ctx, &maps.b, b, b_rows, K))
 				return false;
-			maps.d = maps.e = maps.f = maps.a;
+			maps.d = maps.e = maps.f = maps.dy = maps.w2 = maps.a;
 			p.M = M;
 			p.N = N;
 			p.K = K;
@@ -880,6 +985,22 @@ namespace mb200
 		return with_gate(gate, [&](auto g)
 		{
 			return launch<GATED_BACKWARD, decltype(g)::value>(ctx, maps, p);
+		});
+	}
+
+	bool pair_gated_recompute(mlContext_t ctx, int tokens, int embed, int hidden, const PairOperand &x, const PairOperand &w1, const PairOperand &dy, const PairOperand &w2, int gate, __half *dau,
+			__half *h)
+	{
+		Maps maps;
+		Params p;
+		if (!prepare(ctx, maps, p, tokens, hidden, embed, x, w1, 2 * hidden, BN / 2, 1) || !map_operand(ctx, &maps.dy, dy, tokens, embed) || !map_operand(ctx, &maps.w2, w2, hidden, embed)
+				|| !map_halves(ctx, &maps.d, dau, 2 * hidden, tokens, hidden) || !map_halves(ctx, &maps.e, dau + hidden, 2 * hidden, tokens, hidden)
+				|| !map_halves(ctx, &maps.f, h, hidden, tokens, hidden))
+			return false;
+		p.up_row = hidden;
+		return with_gate(gate, [&](auto g)
+		{
+			return launch<GATED_RECOMPUTE, decltype(g)::value>(ctx, maps, p);
 		});
 	}
 

@@ -45,6 +45,10 @@ namespace mb200
 	 * multiple of 8. */
 	bool pair_gated_backward(mlContext_t ctx, int tokens, int embed, int hidden, const PairOperand &dy, const PairOperand &w2, int gate, const float *au, __half *dau, __half *h);
 
+	/* The same without a kept au: a and u are made again, in the same tiles as dh.  dy [tokens, embed] and w2 stored [embed, hidden] (mn). */
+	bool pair_gated_recompute(mlContext_t ctx, int tokens, int embed, int hidden, const PairOperand &x, const PairOperand &w1, const PairOperand &dy, const PairOperand &w2, int gate, __half *dau,
+			__half *h);
+
 	/* Row statistics of the logits x w^T over columns first .. first + N: parts[t][i] = (maximum, sum of exp(z - maximum)) of group i of
 	 * 128 columns, pair_statistics_parts(N) groups; target_logit[t] where the row's target lies in the range. */
 	int pair_statistics_parts(int N);

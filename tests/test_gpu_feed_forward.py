@@ -70,7 +70,7 @@ def nan_like(t):
 
 
 SIZES = [(1, 64, 64), (2, 256, 40), (5, 128, 1024), (9, 264, 136), (16, 64, 520), (17, 512, 256), (31, 104, 72), (48, 256, 512), (64, 128, 256), (65, 136, 264), (128, 256, 256),
-         (200, 96, 88), (257, 256, 384), (300, 512, 1000), (700, 64, 128), (1025, 320, 264),
+         (200, 96, 88), (257, 256, 384), (300, 1104, 264), (64, 1032, 512), (300, 512, 1000), (700, 64, 128), (1025, 320, 264),
          (1, 67, 33), (3, 33, 130), (40, 35, 71), (130, 65, 129)]
 
 
