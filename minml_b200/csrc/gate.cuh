@@ -10,15 +10,47 @@
 
 namespace mb200
 {
-	template<bool FAST>
-	__device__ __forceinline__ float gate_exp(float x)
+	/* Two fp32 values that one instruction works on (sm_100a: fma, mul and add of register pairs). */
+	struct Pair
 	{
-		return FAST ? __expf(x) : expf(x);
+			float x, y;
+	};
+	__device__ __forceinline__ Pair pair_fma(Pair a, Pair b, Pair c)
+	{
+		Pair d;
+		asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+				: "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+		return d;
 	}
-	template<bool FAST>
-	__device__ __forceinline__ float gate_sigmoid(float g)
-	{ // exp overflows to infinity for large negative g, which gives the right 0
-		return FAST ? __fdividef(1.0f, 1.0f + __expf(-fmaxf(g, -80.0f))) : 1.0f / (1.0f + expf(-g));
+	__device__ __forceinline__ Pair pair_mul(Pair a, Pair b)
+	{
+		Pair d;
+		asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+				: "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+		return d;
+	}
+	__device__ __forceinline__ Pair pair_add(Pair a, Pair b)
+	{
+		Pair d;
+		asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+				: "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+		return d;
+	}
+	__device__ __forceinline__ float reciprocal_approx(float x)
+	{
+		float y;
+		asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+		return y;
+	}
+	/* 1 / (1 + 2^(-g log2 e)): the power overflows to infinity for large negative g, whose reciprocal is the right 0 */
+	__device__ __forceinline__ Pair sigmoid_fast(Pair g)
+	{
+		const Pair t = pair_mul(g, Pair { -1.44269504f, -1.44269504f });
+		Pair e;
+		asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(t.x));
+		asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(t.y));
+		e = pair_add(e, Pair { 1.0f, 1.0f });
+		return Pair { reciprocal_approx(e.x), reciprocal_approx(e.y) };
 	}
 	template<int GATE, bool FAST>
 	__device__ __forceinline__ void gate_with_derivative(float g, float &value, float &derivative)
@@ -32,11 +64,11 @@ namespace mb200
 		{
 			const float phi = 0.5f + 0.5f * erff(g * 0.70710678f);
 			value = g * phi;
-			derivative = phi + 0.39894228f * g * gate_exp<FAST>(-0.5f * g * g);
+			derivative = phi + 0.39894228f * g * (FAST ? __expf(-0.5f * g * g) : expf(-0.5f * g * g));
 		}
 		else
-		{
-			const float s = gate_sigmoid<FAST>(g);
+		{ // exp overflows to infinity for large negative g, which gives the right 0
+			const float s = FAST ? sigmoid_fast(Pair { g, g }).x : 1.0f / (1.0f + expf(-g));
 			value = GATE == MB200_GATE_SIGMOID ? s : g * s;
 			derivative = GATE == MB200_GATE_SIGMOID ? s * (1.0f - s) : s * (1.0f + g * (1.0f - s));
 		}
@@ -46,6 +78,29 @@ namespace mb200
 	{
 		float value, derivative;
 		gate_with_derivative<GATE, FAST>(g, value, derivative);
+		return value;
+	}
+	/* The FAST forms for two values at a time. */
+	template<int GATE>
+	__device__ __forceinline__ void gate_with_derivative(Pair g, Pair &value, Pair &derivative)
+	{
+		if (GATE == MB200_GATE_SILU || GATE == MB200_GATE_SIGMOID)
+		{
+			const Pair s = sigmoid_fast(g), rest = pair_fma(s, Pair { -1.0f, -1.0f }, Pair { 1.0f, 1.0f }); // 1 - s
+			value = GATE == MB200_GATE_SIGMOID ? s : pair_mul(g, s);
+			derivative = GATE == MB200_GATE_SIGMOID ? pair_mul(s, rest) : pair_fma(value, rest, s); // silu: s + g s (1 - s)
+		}
+		else
+		{
+			gate_with_derivative<GATE, true>(g.x, value.x, derivative.x);
+			gate_with_derivative<GATE, true>(g.y, value.y, derivative.y);
+		}
+	}
+	template<int GATE>
+	__device__ __forceinline__ Pair gate_value(Pair g)
+	{
+		Pair value, derivative;
+		gate_with_derivative<GATE>(g, value, derivative);
 		return value;
 	}
 	/* Calls `f` with the gate as a compile-time constant. */

@@ -37,13 +37,10 @@ namespace mb200
 		constexpr int BM = 128; // rows of A per CTA
 		constexpr int BN = 256; // columns of a tile
 		constexpr int BK = 64; // K indices per stage: 128 bytes
-		constexpr int STAGES = 5;
 		constexpr int OPERAND_BYTES = 128 * 128; // one CTA's 128 rows (A) or columns (B) of a stage
 		constexpr int STAGE_BYTES = 2 * OPERAND_BYTES;
 		constexpr int EPI_WARPS = 8;
 		constexpr int THREADS = (2 + EPI_WARPS) * 32;
-		constexpr int STAGING_BYTES = 8192; // per epilogue warp: four 32 x 32 boxes of fp16 or two of fp32
-		constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_WARPS * STAGING_BYTES + 1024;
 		constexpr int HALF_BOX = 32 * 64, FLOAT_BOX = 32 * 128;
 		constexpr int STATISTICS_SEGMENT = 1024 / BK; // K blocks per accumulator in the statistics epilogue
 		constexpr int ROW_GROUP = 8; // tiles of 256 rows that neighbouring clusters share their columns over
@@ -57,6 +54,17 @@ namespace mb200
 			GATED_RECOMPUTE, // the same, with a and u made again in the same tile
 			STATISTICS,
 			PROBABILITIES
+		};
+
+		constexpr int MAX_STAGES = 5;
+		template<int EPI>
+		struct Shape
+		{
+				// per epilogue warp: four 32 x 32 boxes of fp16 or two of fp32; GATED_RECOMPUTE: all six boxes of a tile
+				static constexpr int staging_bytes = EPI == GATED_RECOMPUTE ? 6 * 2048 : 8192;
+				static constexpr int stages = EPI == GATED_RECOMPUTE ? 4 : 5;
+				static constexpr int smem_bytes = stages * STAGE_BYTES + EPI_WARPS * staging_bytes + 1024;
+				static_assert(stages <= MAX_STAGES && smem_bytes <= 227 * 1024, "the configuration exceeds the SM");
 		};
 
 		struct Params
@@ -81,7 +89,7 @@ namespace mb200
 		};
 		struct Barriers
 		{
-				uint64_t full[STAGES], empty[STAGES];
+				uint64_t full[MAX_STAGES], empty[MAX_STAGES];
 				uint64_t tmem_full[2], tmem_empty[2];
 				uint64_t au_empty; // GATED_RECOMPUTE: a and u have been read
 				uint32_t tmem_base;
@@ -136,6 +144,7 @@ namespace mb200
 				const __grid_constant__ CUtensorMap map_d, const __grid_constant__ CUtensorMap map_e, const __grid_constant__ CUtensorMap map_f,
 				const __grid_constant__ CUtensorMap map_dy, const __grid_constant__ CUtensorMap map_w2, const Params p)
 		{
+			constexpr int STAGES = Shape<EPI>::stages;
 			extern __shared__ uint8_t smem_raw[];
 			__shared__ Barriers bars;
 			const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -341,7 +350,7 @@ namespace mb200
 			else
 			{ /* ------------------------------------------------------------ epilogue */
 				const int e = warp - 2, q = warp % 4, half = e / 4;
-				const uint32_t staging = smem_base + STAGES * STAGE_BYTES + e * STAGING_BYTES;
+				const uint32_t staging = smem_base + STAGES * STAGE_BYTES + e * Shape<EPI>::staging_bytes;
 				const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
 				uint32_t buffers = 0, boxes = 0;
 				bool ok = true;
@@ -444,17 +453,19 @@ namespace mb200
 
 					if (EPI == GATED)
 					{
-#pragma unroll 1
+						const int n0 = u.nt * (BN / 2) + half * 64;
+						// h of 64 columns: two boxes; two such pairs take turns, or, where a and u are kept, follow those through the same 8 KB
+						const uint32_t box = staging + (p.keep ? 0 : (boxes++ % 2) * 2 * HALF_BOX);
+						uint32_t packed[2][16];
+#pragma unroll
 						for (int c = 0; c < 2; c++)
 						{
-							const int column = half * 64 + c * 32, n = u.nt * (BN / 2) + column;
+							const int column = half * 64 + c * 32;
 							float a[32], b[32];
 							load_chunk(taddr + column, a);
 							load_chunk(taddr + BN / 2 + column, b);
 							if (c == 1)
 								release();
-							if (n >= p.N)
-								continue; // warp-uniform
 							if (p.keep)
 							{
 								if (lane == 0)
@@ -463,32 +474,45 @@ namespace mb200
 								write_float_box(staging, lane, a);
 								write_float_box(staging + FLOAT_BOX, lane, b);
 								publish();
-								if (lane == 0 && row0 < p.M)
+								if (lane == 0 && row0 < p.M && n0 + c * 32 < p.N)
 								{
-									tma_store_2d(&map_e, staging, n, row0);
-									tma_store_2d(&map_f, staging + FLOAT_BOX, n, row0);
+									tma_store_2d(&map_e, staging, n0 + c * 32, row0);
+									tma_store_2d(&map_f, staging + FLOAT_BOX, n0 + c * 32, row0);
 									bulk_commit_group();
 								}
 							}
 #pragma unroll
-							for (int j = 0; j < 32; j++)
-								a[j] = gate_value<GATE, true>(a[j]) * b[j];
-							if (lane == 0)
+							for (int j = 0; j < 32; j += 2)
 							{
-								if (p.keep)
-									bulk_wait_group_read<0>();
-								else
-									bulk_wait_group_read<3>();
+								const Pair h = pair_mul(gate_value<GATE>(Pair { a[j], a[j + 1] }), Pair { b[j], b[j + 1] });
+								packed[c][j / 2] = pack_half2(h.x, h.y);
 							}
-							__syncwarp();
-							const uint32_t box = staging + (p.keep ? 0 : (boxes++ % 4) * HALF_BOX);
-							write_half_box(box, lane, a);
-							publish();
-							if (lane == 0 && row0 < p.M)
+						}
+						if (lane == 0)
+						{
+							if (p.keep)
+								bulk_wait_group_read<0>();
+							else
+								bulk_wait_group_read<1>();
+						}
+						__syncwarp();
+#pragma unroll
+						for (int c = 0; c < 2; c++)
+#pragma unroll
+							for (int k = 0; k < 4; k++)
+								st_shared_v4(box + c * HALF_BOX + lane * 64 + ((k ^ ((lane >> 1) & 3)) * 16),
+										make_uint4(packed[c][4 * k], packed[c][4 * k + 1], packed[c][4 * k + 2], packed[c][4 * k + 3]));
+						publish();
+						if (lane == 0)
+						{
+							if (row0 < p.M)
 							{
-								tma_store_2d(&map_d, box, n, row0);
-								bulk_commit_group();
+								if (n0 < p.N)
+									tma_store_2d(&map_d, box, n0, row0);
+								if (n0 + 32 < p.N)
+									tma_store_2d(&map_d, box + HALF_BOX, n0 + 32, row0);
 							}
+							bulk_commit_group();
 						}
 						continue;
 					}
@@ -508,42 +532,52 @@ namespace mb200
 						__syncwarp();
 						if (lane == 0)
 							mbar_arrive_cluster(map_to_cta(smem_u32(&bars.au_empty), 0));
+						if (lane == 0)
+							bulk_wait_group_read<0>(); // the boxes of the tile before have left
+						__syncwarp();
+						const int n = u.nt * (BN / 2) + column;
 #pragma unroll
 						for (int c = 0; c < 2; c++)
 						{
-							const int n = u.nt * (BN / 2) + column + c * 32;
-							float v[32], da[32];
+							float v[32];
 							load_chunk(dh + c * 32, v);
 							if (c == 1)
 								release();
-							if (n >= p.N)
-								continue; // warp-uniform
-							if (lane == 0)
-								bulk_wait_group_read<0>();
-							__syncwarp();
+							// eight columns at a time: da, du and h of a row's 16-byte piece
 #pragma unroll
-							for (int j = 0; j < 32; j++)
+							for (int k = 0; k < 4; k++)
 							{
-								float value, derivative;
-								gate_with_derivative<GATE, true>(__uint_as_float(a[c][j]), value, derivative);
-								da[j] = v[j] * __uint_as_float(b[c][j]) * derivative;
-								b[c][j] = __float_as_uint(__uint_as_float(b[c][j]) * value); // h
-								v[j] *= value; // du
-							}
-							write_half_box(staging, lane, da);
-							write_half_box(staging + HALF_BOX, lane, v);
+								float da[8], du[8], h[8];
 #pragma unroll
-							for (int j = 0; j < 32; j++)
-								v[j] = __uint_as_float(b[c][j]);
-							write_half_box(staging + 2 * HALF_BOX, lane, v);
-							publish();
-							if (lane == 0 && row0 < p.M)
-							{
-								tma_store_2d(&map_d, staging, n, row0);
-								tma_store_2d(&map_e, staging + HALF_BOX, n, row0);
-								tma_store_2d(&map_f, staging + 2 * HALF_BOX, n, row0);
-								bulk_commit_group();
+								for (int j = 0; j < 8; j += 2)
+								{
+									const int i = 8 * k + j;
+									const Pair g = { __uint_as_float(a[c][i]), __uint_as_float(a[c][i + 1]) }, up = { __uint_as_float(b[c][i]), __uint_as_float(b[c][i + 1]) }, d = { v[i], v[i + 1] };
+									Pair value, derivative;
+									gate_with_derivative<GATE>(g, value, derivative);
+									const Pair x = pair_mul(d, pair_mul(up, derivative)), y = pair_mul(d, value), z = pair_mul(up, value);
+									da[j] = x.x, da[j + 1] = x.y;
+									du[j] = y.x, du[j + 1] = y.y;
+									h[j] = z.x, h[j + 1] = z.y;
+								}
+								const uint32_t at = staging + c * 3 * HALF_BOX + lane * 64 + ((k ^ ((lane >> 1) & 3)) * 16);
+								st_shared_v4(at, pack_half8(da));
+								st_shared_v4(at + HALF_BOX, pack_half8(du));
+								st_shared_v4(at + 2 * HALF_BOX, pack_half8(h));
 							}
+						}
+						publish();
+						if (lane == 0 && row0 < p.M)
+						{
+#pragma unroll
+							for (int c = 0; c < 2; c++)
+								if (n + c * 32 < p.N)
+								{
+									tma_store_2d(&map_d, staging + c * 3 * HALF_BOX, n + c * 32, row0);
+									tma_store_2d(&map_e, staging + (c * 3 + 1) * HALF_BOX, n + c * 32, row0);
+									tma_store_2d(&map_f, staging + (c * 3 + 2) * HALF_BOX, n + c * 32, row0);
+								}
+							bulk_commit_group();
 						}
 						continue;
 					}
@@ -576,13 +610,15 @@ namespace mb200
 								bulk_wait_group_read<0>();
 							__syncwarp();
 #pragma unroll
-							for (int j = 0; j < 32; j++)
+							for (int j = 0; j < 32; j += 2)
 							{
-								float value, derivative;
-								gate_with_derivative<GATE, true>(a[j], value, derivative);
-								a[j] = v[j] * b[j] * derivative;
-								b[j] *= value; // h
-								v[j] *= value; // du
+								const Pair up = { b[j], b[j + 1] }, d = { v[j], v[j + 1] };
+								Pair value, derivative;
+								gate_with_derivative<GATE>(Pair { a[j], a[j + 1] }, value, derivative);
+								const Pair x = pair_mul(d, pair_mul(up, derivative)), y = pair_mul(d, value), z = pair_mul(up, value);
+								a[j] = x.x, a[j + 1] = x.y; // da
+								v[j] = y.x, v[j + 1] = y.y; // du
+								b[j] = z.x, b[j + 1] = z.y; // h
 							}
 							write_half_box(staging, lane, a);
 							write_half_box(staging + HALF_BOX, lane, v);
@@ -718,10 +754,10 @@ namespace mb200
 				attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
 				config.gridDim = dim3(2 * (get(ctx)->sm_count / 2));
 				config.blockDim = dim3(THREADS);
-				config.dynamicSmemBytes = SMEM_BYTES;
+				config.dynamicSmemBytes = Shape<EPI>::smem_bytes;
 				config.attrs = &attribute;
 				config.numAttrs = 1;
-				if (cudaFuncSetAttribute(kernel_gemm_pair<EPI, GATE>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess
+				if (cudaFuncSetAttribute(kernel_gemm_pair<EPI, GATE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<EPI>::smem_bytes) != cudaSuccess
 						|| cudaOccupancyMaxActiveClusters(&n, kernel_gemm_pair<EPI, GATE>, &config) != cudaSuccess || n <= 0)
 				{
 					cudaGetLastError();
@@ -742,7 +778,7 @@ namespace mb200
 			const int resident = resident_clusters<EPI, GATE>(ctx);
 			if (resident == 0)
 			{
-				record_error(ctx, "gemm_pair: a cluster of two CTAs with %d bytes of shared memory each cannot be placed on this device", SMEM_BYTES);
+				record_error(ctx, "gemm_pair: a cluster of two CTAs with %d bytes of shared memory each cannot be placed on this device", Shape<EPI>::smem_bytes);
 				return false;
 			}
 			Context *c = get(ctx);
@@ -757,7 +793,7 @@ namespace mb200
 			attributes[1].val.programmaticStreamSerializationAllowed = 1;
 			config.gridDim = dim3(2 * std::min(units, resident));
 			config.blockDim = dim3(THREADS);
-			config.dynamicSmemBytes = SMEM_BYTES;
+			config.dynamicSmemBytes = Shape<EPI>::smem_bytes;
 			config.stream = use_stream(ctx);
 			config.attrs = attributes;
 			config.numAttrs = 2;
