@@ -115,6 +115,13 @@ namespace mb200
 					:: "l"(reinterpret_cast<uint64_t>(map)), "r"(src), "r"(c0), "r"(c1) : "memory");
 		}
 
+		/* On the even CTA's barrier.  What it reports is that tensor memory has been read (ordered by tcgen05.fence), no memory write: a release at
+		 * cluster scope would wait for every store of the thread, measured as the largest stall of the short-K epilogues. */
+		__device__ __forceinline__ void arrive_at_leader(uint32_t bar)
+		{
+			asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" :: "r"(map_to_cta(bar, 0)) : "memory");
+		}
+
 		/* A warp's 32 x 32 boxes in shared memory: a lane owns one row.  fp16: 64-byte rows, 16-byte piece k at k ^ (row / 2 % 4) (64-byte
 		 * swizzle); fp32: 128-byte rows, piece k at k ^ (row % 8) (128-byte swizzle). */
 		__device__ __forceinline__ void write_half_box(uint32_t box, int lane, const float (&v)[32])
@@ -280,7 +287,7 @@ namespace mb200
 						if (EPI == GATED_RECOMPUTE)
 						{ // dh into columns 256 + 128 i, two buffers; a and u, below, into columns 0 .. 255
 							const uint32_t acc = buffers & 1u;
-							if (!mbar_wait_cluster(smem_u32(&bars.tmem_empty[acc]), ((buffers >> 1) & 1u) ^ 1u, abort_flag))
+							if (!mbar_wait(smem_u32(&bars.tmem_empty[acc]), ((buffers >> 1) & 1u) ^ 1u, abort_flag))
 								break;
 							tcgen05_fence_after();
 							const uint32_t idesc_dh = make_idesc_f16_pair(BN / 2) | (1u << 16);
@@ -300,7 +307,7 @@ namespace mb200
 									mma_ss_pair<0>(tmem_base + BN + acc * (BN / 2), desc_a + 2 * k, desc_b + 128 * k, idesc_dh, kb > u.kb0 || k > 0 ? 1u : 0u);
 								mma_commit_pair(smem_u32(&bars.empty[s]));
 							}
-							if (!ok || !mbar_wait_cluster(smem_u32(&bars.au_empty), (buffers & 1u) ^ 1u, abort_flag))
+							if (!ok || !mbar_wait(smem_u32(&bars.au_empty), (buffers & 1u) ^ 1u, abort_flag))
 								break;
 							tcgen05_fence_after();
 						}
@@ -310,7 +317,7 @@ namespace mb200
 							const uint32_t acc = buffers & 1u;
 							if (EPI != GATED_RECOMPUTE)
 							{
-								if (!mbar_wait_cluster(smem_u32(&bars.tmem_empty[acc]), ((buffers >> 1) & 1u) ^ 1u, abort_flag))
+								if (!mbar_wait(smem_u32(&bars.tmem_empty[acc]), ((buffers >> 1) & 1u) ^ 1u, abort_flag))
 								{
 									ok = false;
 									break;
@@ -366,7 +373,7 @@ namespace mb200
 					tcgen05_fence_before();
 					__syncwarp();
 					if (lane == 0)
-						mbar_arrive_cluster(map_to_cta(smem_u32(&bars.tmem_empty[buffers & 1u]), 0));
+						arrive_at_leader(smem_u32(&bars.tmem_empty[buffers & 1u]));
 					buffers++;
 				};
 				auto publish = [&]()
@@ -531,7 +538,7 @@ namespace mb200
 						tcgen05_fence_before();
 						__syncwarp();
 						if (lane == 0)
-							mbar_arrive_cluster(map_to_cta(smem_u32(&bars.au_empty), 0));
+							arrive_at_leader(smem_u32(&bars.au_empty));
 						if (lane == 0)
 							bulk_wait_group_read<0>(); // the boxes of the tile before have left
 						__syncwarp();
