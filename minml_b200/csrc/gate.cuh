@@ -42,15 +42,18 @@ namespace mb200
 		asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
 		return y;
 	}
-	/* 1 / (1 + 2^(-g log2 e)): the power overflows to infinity for large negative g, whose reciprocal is the right 0 */
+	/* 1 / (1 + 2^(-g log2 e)) of two values with one reciprocal, 1 / a = b / (a b): the special-function unit is what an epilogue with this gate
+	 * runs out of first (three instead of four of its instructions for two values).  The power is held at 2^60 so that the product stays
+	 * finite: a sigmoid below 2^-60 comes out as 2^-60, which fp16 rounds to the same 0. */
 	__device__ __forceinline__ Pair sigmoid_fast(Pair g)
 	{
 		const Pair t = pair_mul(g, Pair { -1.44269504f, -1.44269504f });
 		Pair e;
-		asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(t.x));
-		asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(t.y));
+		asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(fminf(t.x, 60.0f)));
+		asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(fminf(t.y, 60.0f)));
 		e = pair_add(e, Pair { 1.0f, 1.0f });
-		return Pair { reciprocal_approx(e.x), reciprocal_approx(e.y) };
+		const float r = reciprocal_approx(e.x * e.y);
+		return pair_mul(Pair { r, r }, Pair { e.y, e.x });
 	}
 	template<int GATE, bool FAST>
 	__device__ __forceinline__ void gate_with_derivative(float g, float &value, float &derivative)
@@ -68,7 +71,7 @@ namespace mb200
 		}
 		else
 		{ // exp overflows to infinity for large negative g, which gives the right 0
-			const float s = FAST ? sigmoid_fast(Pair { g, g }).x : 1.0f / (1.0f + expf(-g));
+			const float s = FAST ? __fdividef(1.0f, 1.0f + __expf(-g)) : 1.0f / (1.0f + expf(-g));
 			value = GATE == MB200_GATE_SIGMOID ? s : g * s;
 			derivative = GATE == MB200_GATE_SIGMOID ? s * (1.0f - s) : s * (1.0f + g * (1.0f - s));
 		}
@@ -87,7 +90,8 @@ namespace mb200
 		if (GATE == MB200_GATE_SILU || GATE == MB200_GATE_SIGMOID)
 		{
 			const Pair s = sigmoid_fast(g), rest = pair_fma(s, Pair { -1.0f, -1.0f }, Pair { 1.0f, 1.0f }); // 1 - s
-			value = GATE == MB200_GATE_SIGMOID ? s : pair_mul(g, s);
+			// (a NaN has passed sigmoid_fast as if it were large)
+			value = GATE == MB200_GATE_SIGMOID ? Pair { g.x == g.x ? s.x : g.x, g.y == g.y ? s.y : g.y } : pair_mul(g, s);
 			derivative = GATE == MB200_GATE_SIGMOID ? pair_mul(s, rest) : pair_fma(value, rest, s); // silu: s + g s (1 - s)
 		}
 		else

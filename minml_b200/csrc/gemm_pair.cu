@@ -8,7 +8,7 @@
  * run under the multiplications of the next.
  *   warp 0      fetches this CTA's A and B boxes by TMA into a ring of stages of 64 K indices (128-byte rows, 128-byte swizzle)
  *   warp 1      in the even CTA: issues the multiplications; owns the tensor-memory allocation
- *   warps 2-9   epilogue: two warps per tensor-memory lane quarter, each half of the columns
+ *   warps 4-11  epilogue: two warps per tensor-memory lane quarter, each half of the columns
  * An operand stored [K, rows] is fetched in boxes of 64 K indices x 64 rows and read as an MN-major operand.
  * K and row tails are zero-filled by TMA, results are clipped by their tensor maps.
  *
@@ -40,7 +40,10 @@ namespace mb200
 		constexpr int OPERAND_BYTES = 128 * 128; // one CTA's 128 rows (A) or columns (B) of a stage
 		constexpr int STAGE_BYTES = 2 * OPERAND_BYTES;
 		constexpr int EPI_WARPS = 8;
-		constexpr int THREADS = (2 + EPI_WARPS) * 32;
+		constexpr int EPI_FIRST = 4; // first epilogue warp: registers are moved between groups of four warps
+		constexpr int THREADS = (EPI_FIRST + EPI_WARPS) * 32;
+		// of the 168 registers a thread starts with, what the first four warps give up is what the epilogue gets: 128 * 40 + 256 * 232 = 384 * 168
+		constexpr int REGISTERS_FEW = 40, REGISTERS_MANY = 232;
 		constexpr int HALF_BOX = 32 * 64, FLOAT_BOX = 32 * 128;
 		constexpr int STATISTICS_SEGMENT = 1024 / BK; // K blocks per accumulator in the statistics epilogue
 		constexpr int ROW_GROUP = 8; // tiles of 256 rows that neighbouring clusters share their columns over
@@ -63,6 +66,7 @@ namespace mb200
 				// per epilogue warp: four 32 x 32 boxes of fp16 or two of fp32; GATED_RECOMPUTE: all six boxes of a tile
 				static constexpr int staging_bytes = EPI == GATED_RECOMPUTE ? 6 * 2048 : 8192;
 				static constexpr int stages = EPI == GATED_RECOMPUTE ? 4 : 5;
+				static constexpr bool moves_registers = EPI == GATED_RECOMPUTE || EPI == STATISTICS; // they hold 128 accumulators a thread
 				static constexpr int smem_bytes = stages * STAGE_BYTES + EPI_WARPS * staging_bytes + 1024;
 				static_assert(stages <= MAX_STAGES && smem_bytes <= 227 * 1024, "the configuration exceeds the SM");
 		};
@@ -212,8 +216,14 @@ namespace mb200
 			let_next_grid_start();
 			wait_for_previous_grid();
 
+			auto give_registers = [&]()
+			{
+				if (Shape<EPI>::moves_registers)
+					asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(REGISTERS_FEW));
+			};
 			if (warp == 0)
 			{ /* ------------------------------------------------ operands */
+				give_registers();
 				if (elect_one())
 				{
 					prefetch_tensormap(&map_a);
@@ -274,6 +284,7 @@ namespace mb200
 			}
 			else if (warp == 1)
 			{ /* ------------------------------------------- multiplications */
+				give_registers();
 				if (leader && elect_one())
 				{
 					const uint32_t idesc = make_idesc_f16_pair(BN) | (p.a_mn ? (1u << 15) : 0u) | (p.b_mn ? (1u << 16) : 0u);
@@ -354,9 +365,13 @@ namespace mb200
 				}
 				__syncwarp();
 			}
+			else if (warp < EPI_FIRST)
+				give_registers();
 			else
 			{ /* ------------------------------------------------------------ epilogue */
-				const int e = warp - 2, q = warp % 4, half = e / 4;
+				if (Shape<EPI>::moves_registers)
+					asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(REGISTERS_MANY));
+				const int e = warp - EPI_FIRST, q = warp % 4, half = e / 4;
 				const uint32_t staging = smem_base + STAGES * STAGE_BYTES + e * Shape<EPI>::staging_bytes;
 				const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
 				uint32_t buffers = 0, boxes = 0;
