@@ -80,20 +80,34 @@ namespace mb200
 				long long tokens, int first, int width, bool last, float *__restrict__ loss, float *__restrict__ lse)
 		{
 			__shared__ float2 scratch[8];
+			wait_for_previous_grid();
 			for (long long t = blockIdx.x; t < tokens; t += gridDim.x)
 			{
 				const float *row = z + t * pitch;
 				float2 mine = make_float2(-INFINITY, 0.0f);
-				for (int c = threadIdx.x; c < width; c += 256)
-				{
-					const float v = row[c];
-					if (v > mine.x)
+				for (int c = threadIdx.x * 4; c < width; c += 256 * 4 * 4)
+				{ // sixteen values at a time: their maximum, then their exponentials (rows are padded to a multiple of 64 floats)
+					float4 v[4];
+					float top = -INFINITY;
+#pragma unroll
+					for (int k = 0; k < 4; k++)
 					{
-						mine.y = mine.y * expf(mine.x - v) + 1.0f;
-						mine.x = v;
+						const int at = c + k * 1024;
+						v[k] = at < width ? *reinterpret_cast<const float4*>(row + at) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+						if (at + 1 >= width)
+							v[k].y = -INFINITY;
+						if (at + 2 >= width)
+							v[k].z = -INFINITY;
+						if (at + 3 >= width)
+							v[k].w = -INFINITY;
+						top = fmaxf(top, fmaxf(fmaxf(v[k].x, v[k].y), fmaxf(v[k].z, v[k].w))); // a NaN gives way to a number here and reaches the sum
 					}
-					else
-						mine.y += mine.x == v && v == -INFINITY ? 0.0f : expf(v - mine.x); // a NaN reaches the sum
+					const float shift = top == -INFINITY ? 0.0f : top;
+					float sum = 0.0f;
+#pragma unroll
+					for (int k = 0; k < 4; k++)
+						sum += (expf(v[k].x - shift) + expf(v[k].y - shift)) + (expf(v[k].z - shift) + expf(v[k].w - shift));
+					mine = merge(mine, make_float2(top, sum));
 				}
 				mine = merge_warp(mine);
 				if (threadIdx.x % 32 == 0)
@@ -116,16 +130,26 @@ namespace mb200
 			}
 		}
 
-		/* z becomes exp(z - lse) - [target] for one piece; rows that take no part are zero */
-		__global__ void __launch_bounds__(256) kernel_piece_gradient(float *__restrict__ z, int pitch, const float *__restrict__ lse, Rows rows, long long tokens, int first, int width)
+		/* z becomes alpha c_t (exp(z - lse) - [target]) for one piece, four columns a thread; rows that take no part are zero */
+		__global__ void __launch_bounds__(256) kernel_piece_gradient(float *__restrict__ z, int pitch, const float *__restrict__ lse, Rows rows, long long tokens, int first, int width,
+				float alpha)
 		{
-			const long long total = tokens * width, stride = static_cast<long long>(gridDim.x) * 256;
+			wait_for_previous_grid();
+			const int groups = (width + 3) / 4;
+			const long long total = tokens * groups, stride = static_cast<long long>(gridDim.x) * 256;
 			for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < total; i += stride)
 			{
-				const long long t = i / width;
-				const int c = static_cast<int>(i - t * width);
-				const float v = expf(z[t * pitch + c] - lse[t]) - (rows.targets[t] - first == c ? 1.0f : 0.0f);
-				z[t * pitch + c] = rows.weight(t) != 0.0f ? v : 0.0f;
+				const long long t = i / groups;
+				const int c = static_cast<int>(i - t * groups) * 4, target = rows.targets[t] - first - c;
+				const float weight = rows.weight(t), l = lse[t], factor = alpha * weight;
+				float4 *at = reinterpret_cast<float4*>(z + t * pitch + c);
+				float4 v = *at;
+				if (weight == 0.0f)
+					v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+				else
+					v = make_float4(factor * (expf(v.x - l) - (target == 0 ? 1.0f : 0.0f)), factor * (expf(v.y - l) - (target == 1 ? 1.0f : 0.0f)),
+							factor * (expf(v.z - l) - (target == 2 ? 1.0f : 0.0f)), factor * (expf(v.w - l) - (target == 3 ? 1.0f : 0.0f)));
+				*at = v;
 			}
 		}
 
@@ -150,14 +174,14 @@ namespace mb200
 					out[0] = m;
 			}
 		}
-		/* x times c_t / max |c|; zero in the rows that take no part, whatever they hold */
+		/* x, times c_t / max |c| where weights are `applied`; zero in the rows that take no part, whatever they hold */
 		template<typename T>
-		__global__ void __launch_bounds__(256) kernel_weighted_rows(T *__restrict__ out, const T *__restrict__ x, Rows rows, const float *__restrict__ largest, long long tokens,
-				int embed)
+		__global__ void __launch_bounds__(256) kernel_weighted_rows(T *__restrict__ out, const T *__restrict__ x, Rows rows, bool applied, const float *__restrict__ largest,
+				long long tokens, int embed)
 		{
 			for (long long t = blockIdx.x; t < tokens; t += gridDim.x)
 			{
-				const float c = rows.weight(t), factor = c == 0.0f ? 0.0f : largest == nullptr ? c : c / largest[0];
+				const float c = rows.weight(t), factor = c == 0.0f ? 0.0f : largest != nullptr ? c / largest[0] : applied ? c : 1.0f;
 				for (int k = threadIdx.x; k < embed; k += 256)
 					out[t * embed + k] = factor == 0.0f ? from_float<T>(0.0f) : from_float<T>(to_float(x[t * embed + k]) * factor);
 			}
@@ -206,7 +230,7 @@ namespace mb200
 				int piece, pitch; // columns of a piece of logits or probabilities, and its rows' pitch
 				int dx_splits; // fp32 sums that dx is kept in until the last piece
 				float2 *running = nullptr; // fp32: per row; fp16: per row and 128 columns
-				float *target_logit = nullptr, *z = nullptr, *dx_sums = nullptr, *dw_sum = nullptr, *partials = nullptr, *largest = nullptr;
+				float *target_logit = nullptr, *z = nullptr, *dx_sums = nullptr, *partials = nullptr, *largest = nullptr;
 				void *p = nullptr, *x = nullptr, *w = nullptr, *weighted_x = nullptr;
 				size_t bytes = 0;
 				Plan(mlContext_t ctx, const Problem &q, void *workspace, bool training, int columns)
@@ -236,9 +260,7 @@ namespace mb200
 						largest = carve.take<float>(1);
 						weighted_x = carve.take<uint8_t>(rows * es);
 						p = half ? carve.take<uint8_t>(cells * es) : nullptr; // fp32: in place of the logits
-						dx_sums = carve.take<float>(rows * dx_splits);
-						if (!half) // dW of a piece, to which a factor that only the device knows is applied
-							dw_sum = carve.take<float>(static_cast<size_t>(piece) * embed);
+						dx_sums = half ? carve.take<float>(rows * dx_splits) : nullptr;
 					}
 					// products that are cut along K: of a whole piece, and of the last, narrower one
 					size_t partial = 0;
@@ -365,11 +387,12 @@ namespace mb200
 				if (!float_product(ctx, static_cast<int>(q.tokens), width, q.embed, FloatOperand { o.x, plan.embed, false },
 						FloatOperand { o.w + static_cast<size_t>(first) * plan.embed, plan.embed, false }, plan.z, plan.pitch, 0.0f, plan.partials))
 					return;
-				kernel_piece_statistics<<<row_blocks(ctx, q.tokens), 256, 0, use_stream(ctx)>>>(plan.z, plan.pitch, plan.running, plan.target_logit, rows, q.tokens, first, width,
-						first + width == q.vocab, loss, lse);
+				const cudaError_t status = launch_overlapped(kernel_piece_statistics, dim3(row_blocks(ctx, q.tokens)), dim3(256), 0, use_stream(ctx), plan.z, plan.pitch, plan.running,
+						plan.target_logit, rows, q.tokens, first, width, first + width == q.vocab, loss, lse);
 				MB200_COUNT_LAUNCH();
+				if (!check_cuda(ctx, status, "mb200_softmax_cross_entropy_forward"))
+					return;
 			}
-			check_cuda(ctx, cudaGetLastError(), "mb200_softmax_cross_entropy_forward");
 		}
 		template<typename T>
 		void backward(mlContext_t ctx, const Problem &q, const Rows &rows, const Plan &plan, const Operands<T> &o, const float *lse, float alpha, float beta_dx, T *dx, float beta_dw, T *dw)
@@ -377,8 +400,9 @@ namespace mb200
 			cudaStream_t stream = use_stream(ctx);
 			constexpr bool half = sizeof(T) == 2;
 			const int tokens = static_cast<int>(q.tokens), D = q.embed, ld = plan.embed;
-			const float unscale = half ? alpha / P_SCALE : alpha;
-			const float *largest = rows.weights == nullptr ? nullptr : plan.largest;
+			// fp16: factors go into results and the copy of x (see above); fp32 has the range to take them all into P, and the copy only masks rows
+			const float unscale = alpha / P_SCALE;
+			const float *largest = half && rows.weights != nullptr ? plan.largest : nullptr;
 			if (dw != nullptr)
 			{
 				if (largest != nullptr)
@@ -386,7 +410,7 @@ namespace mb200
 					kernel_largest_weight<<<1, 1024, 0, stream>>>(plan.largest, rows, q.tokens);
 					MB200_COUNT_LAUNCH();
 				}
-				kernel_weighted_rows<T> <<<row_blocks(ctx, q.tokens), 256, 0, stream>>>(reinterpret_cast<T*>(plan.weighted_x), o.x, rows, largest, q.tokens, ld);
+				kernel_weighted_rows<T> <<<row_blocks(ctx, q.tokens), 256, 0, stream>>>(reinterpret_cast<T*>(plan.weighted_x), o.x, rows, half, largest, q.tokens, ld);
 				MB200_COUNT_LAUNCH();
 				if (!check_cuda(ctx, cudaGetLastError(), "mb200_softmax_cross_entropy_backward: row weights"))
 					return;
@@ -413,21 +437,23 @@ namespace mb200
 				{
 					if (!float_product(ctx, tokens, width, D, FloatOperand { o.x, ld, false }, FloatOperand { w, ld, false }, plan.z, plan.pitch, 0.0f, plan.partials))
 						return;
-					kernel_piece_gradient<<<elementwise_blocks(ctx, q.tokens * width), 256, 0, stream>>>(plan.z, plan.pitch, lse, rows, q.tokens, first, width);
+					const cudaError_t status = launch_overlapped(kernel_piece_gradient, dim3(elementwise_blocks(ctx, q.tokens * ((width + 3) / 4))), dim3(256), 0, stream, plan.z, plan.pitch, lse,
+							rows, q.tokens, first, width, alpha);
 					MB200_COUNT_LAUNCH();
-					if (!check_cuda(ctx, cudaGetLastError(), "mb200_softmax_cross_entropy_backward: probabilities"))
+					if (!check_cuda(ctx, status, "mb200_softmax_cross_entropy_backward: probabilities"))
 						return;
 					if (dx != nullptr
-							&& !float_product(ctx, tokens, D, width, FloatOperand { plan.z, plan.pitch, false }, FloatOperand { w, ld, true }, plan.dx_sums, ld, first > 0 ? 1.0f : 0.0f, plan.partials))
+							&& !float_product(ctx, tokens, D, width, FloatOperand { plan.z, plan.pitch, false }, FloatOperand { w, ld, true }, dx, D, first > 0 ? 1.0f : beta_dx, plan.partials))
 						return;
 					if (dw != nullptr
-							&& (!float_product(ctx, width, D, tokens, FloatOperand { plan.z, plan.pitch, true }, FloatOperand { weighted_x, ld, true }, plan.dw_sum, ld, 0.0f, plan.partials)
-									|| !finish_sums<float>(ctx, dw + static_cast<size_t>(first) * D, D, width, D, plan.dw_sum, ld, 1, unscale, largest, nullptr, beta_dw)))
+							&& !float_product(ctx, width, D, tokens, FloatOperand { plan.z, plan.pitch, true }, FloatOperand { weighted_x, ld, true }, dw + static_cast<size_t>(first) * D, D,
+									beta_dw, plan.partials))
 						return;
 				}
 			}
-			if (dx != nullptr)
-				finish_sums<T>(ctx, dx, D, tokens, D, plan.dx_sums, ld, plan.dx_splits, unscale, nullptr, rows.weights, beta_dx);
+			if constexpr (half)
+				if (dx != nullptr)
+					finish_sums<T>(ctx, dx, D, tokens, D, plan.dx_sums, ld, plan.dx_splits, unscale, nullptr, rows.weights, beta_dx);
 		}
 	}
 } /* namespace mb200 */

@@ -24,37 +24,80 @@ namespace mb200
 {
 	namespace
 	{
-		/* h = act(a) u from the pre-activations au [tokens, 2 hidden], fp32 */
-		template<typename T, int GATE>
-		__global__ void __launch_bounds__(256) kernel_gate(T *__restrict__ h, const float *__restrict__ au, long long tokens, int hidden)
+		/* The gate between two fp32 products.  Four hidden units a thread; a and u lie `up` floats apart in rows of 2 up (up is hidden, or hidden
+		 * without its padding in a kept au, whose rows may start anywhere); the padding's a and u count as zero. */
+		struct alignas(16) Four
 		{
-			const long long total = tokens * hidden, stride = static_cast<long long>(gridDim.x) * 256;
+				float v[4];
+		};
+		__device__ __forceinline__ void load_pre_activations(Four &a, Four &u, const float *__restrict__ au, long long token, int column, int up)
+		{
+			const float *src = au + token * 2 * up + column;
+			if (up % 4 == 0)
+			{
+				a = *reinterpret_cast<const Four*>(src);
+				u = *reinterpret_cast<const Four*>(src + up);
+				return;
+			}
+#pragma unroll
+			for (int k = 0; k < 4; k++)
+			{
+				a.v[k] = column + k < up ? src[k] : 0.0f;
+				u.v[k] = column + k < up ? src[up + k] : 0.0f;
+			}
+		}
+		template<int GATE>
+		__global__ void __launch_bounds__(256) kernel_gate(float *__restrict__ h, const float *__restrict__ au, long long tokens, int hidden, int up)
+		{
+			let_next_grid_start();
+			wait_for_previous_grid();
+			const int groups = hidden / 4;
+			const long long total = tokens * groups, stride = static_cast<long long>(gridDim.x) * 256;
 			for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < total; i += stride)
 			{
-				const long long t = i / hidden, at = t * 2 * hidden + (i - t * hidden);
-				h[i] = from_float<T>(gate_value<GATE, false>(au[at]) * au[at + hidden]);
+				const long long t = i / groups;
+				const int c = static_cast<int>(i - t * groups) * 4;
+				Four a, u;
+				load_pre_activations(a, u, au, t, c, up);
+#pragma unroll
+				for (int k = 0; k < 4; k++)
+					u.v[k] *= gate_value<GATE, false>(a.v[k]);
+				*reinterpret_cast<Four*>(h + t * hidden + c) = u;
 			}
 		}
 		/* [da du] and h from dh [tokens, hidden] and the pre-activations */
-		template<typename T, int GATE>
-		__global__ void __launch_bounds__(256) kernel_gate_backward(T *__restrict__ dau, T *__restrict__ h, const float *__restrict__ dh, const float *__restrict__ au,
-				long long tokens, int hidden)
+		template<int GATE>
+		__global__ void __launch_bounds__(256) kernel_gate_backward(float *__restrict__ dau, float *__restrict__ h, const float *__restrict__ dh, const float *__restrict__ au, long long tokens,
+				int hidden, int up)
 		{
-			const long long total = tokens * hidden, stride = static_cast<long long>(gridDim.x) * 256;
+			let_next_grid_start();
+			wait_for_previous_grid();
+			const int groups = hidden / 4;
+			const long long total = tokens * groups, stride = static_cast<long long>(gridDim.x) * 256;
 			for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < total; i += stride)
 			{
-				const long long t = i / hidden, at = t * 2 * hidden + (i - t * hidden);
-				float value, derivative;
-				gate_with_derivative<GATE, false>(au[at], value, derivative);
-				const float u = au[at + hidden], d = dh[i];
-				dau[at] = from_float<T>(d * u * derivative);
-				dau[at + hidden] = from_float<T>(d * value);
-				h[i] = from_float<T>(value * u);
+				const long long t = i / groups;
+				const int c = static_cast<int>(i - t * groups) * 4;
+				Four a, u, d = *reinterpret_cast<const Four*>(dh + t * hidden + c);
+				load_pre_activations(a, u, au, t, c, up);
+#pragma unroll
+				for (int k = 0; k < 4; k++)
+				{
+					float value, derivative;
+					gate_with_derivative<GATE, false>(a.v[k], value, derivative);
+					a.v[k] = d.v[k] * u.v[k] * derivative;
+					d.v[k] *= value;
+					u.v[k] *= value;
+				}
+				float *dst = dau + t * 2 * hidden + c;
+				*reinterpret_cast<Four*>(dst) = a;
+				*reinterpret_cast<Four*>(dst + hidden) = d;
+				*reinterpret_cast<Four*>(h + t * hidden + c) = u;
 			}
 		}
 		int elementwise_blocks(mlContext_t ctx, long long elements)
 		{
-			return static_cast<int>(std::max<long long>(1, std::min<long long>((elements + 255) / 256, static_cast<long long>(get(ctx)->sm_count) * 8)));
+			return static_cast<int>(std::max<long long>(1, std::min<long long>((elements + 255) / 256, static_cast<long long>(get(ctx)->sm_count) * 16)));
 		}
 
 		struct Problem
@@ -71,7 +114,7 @@ namespace mb200
 		{
 				int embed, hidden; // padded
 				bool pack_x, pack_w1, pack_w2;
-				bool keeps; // what the forward pass leaves in `saved` is used: its rows can be addressed
+				bool keeps; // what the forward pass leaves in `saved` is used
 				void *x = nullptr, *w1 = nullptr, *w2 = nullptr, *dy = nullptr, *h = nullptr, *dau = nullptr;
 				float *au = nullptr, *dh = nullptr, *partials = nullptr;
 				size_t bytes = 0;
@@ -85,7 +128,7 @@ namespace mb200
 					pack_x = embed != p.embed;
 					pack_w1 = pack_x || hidden != p.hidden;
 					pack_w2 = hidden != p.hidden;
-					keeps = saved && hidden == p.hidden && (p.dtype == DTYPE_FLOAT32 || p.embed > RECOMPUTE_UP_TO);
+					keeps = saved && (p.dtype == DTYPE_FLOAT32 || (hidden == p.hidden && p.embed > RECOMPUTE_UP_TO));
 					const size_t th = static_cast<size_t>(p.tokens) * hidden, te = static_cast<size_t>(p.tokens) * embed;
 					if (pack_x)
 						x = carve.take<uint8_t>(te * es);
@@ -102,7 +145,7 @@ namespace mb200
 					};
 					size_t partial = cut(tokens, p.embed, hidden); // y
 					if (p.dtype == DTYPE_FLOAT32)
-						partial = std::max(partial, cut(tokens, 2 * hidden, p.embed));
+						partial = std::max( { partial, cut(tokens, 2 * hidden, p.embed), cut(tokens, p.hidden, p.embed) });
 					if (backward)
 					{
 						if (pack_x)
@@ -163,16 +206,24 @@ namespace mb200
 								reinterpret_cast<__half*>(plan.h), plan.hidden, au);
 					else
 					{
-						if (!product(tokens, 2 * plan.hidden, p.embed, x, plan.embed, false, w1, plan.embed, false, au, 2 * plan.hidden, 0.0f))
-							return false;
+						// one product, or two where the rows of a kept au have no padding between a and u
+						const int up = up_offset(), parts = up == plan.hidden ? 1 : 2;
+						for (int i = 0; i < parts; i++)
+							if (!product(tokens, 2 * up / parts, p.embed, x, plan.embed, false, w1 + static_cast<size_t>(i) * plan.hidden * plan.embed, plan.embed, false, au + i * up, 2 * up, 0.0f))
+								return false;
+						cudaError_t status = cudaSuccess;
 						with_gate(p.gate, [&](auto gate)
 						{
-							kernel_gate<T, decltype(gate)::value> <<<elementwise_blocks(ctx, p.tokens * plan.hidden), 256, 0, use_stream(ctx)>>>(reinterpret_cast<T*>(plan.h), au,
-									p.tokens, plan.hidden);
+							status = launch_overlapped(kernel_gate<decltype(gate)::value>, dim3(elementwise_blocks(ctx, p.tokens * plan.hidden / 4)), dim3(256), 0, use_stream(ctx),
+									reinterpret_cast<float*>(plan.h), au, p.tokens, plan.hidden, up);
 						});
 						MB200_COUNT_LAUNCH();
-						return check_cuda(ctx, cudaGetLastError(), "gated feed-forward: gate");
+						return check_cuda(ctx, status, "gated feed-forward: gate");
 					}
+				}
+				int up_offset() const
+				{
+					return plan.keeps ? p.hidden : plan.hidden;
 				}
 				bool gate_backward(const float *au)
 				{
@@ -187,13 +238,14 @@ namespace mb200
 					{
 						if (!product(tokens, plan.hidden, p.embed, dy, plan.embed, false, w2, plan.hidden, true, plan.dh, plan.hidden, 0.0f))
 							return false;
+						cudaError_t status = cudaSuccess;
 						with_gate(p.gate, [&](auto gate)
 						{
-							kernel_gate_backward<T, decltype(gate)::value> <<<elementwise_blocks(ctx, p.tokens * plan.hidden), 256, 0, use_stream(ctx)>>>(
-									reinterpret_cast<T*>(plan.dau), reinterpret_cast<T*>(plan.h), plan.dh, au, p.tokens, plan.hidden);
+							status = launch_overlapped(kernel_gate_backward<decltype(gate)::value>, dim3(elementwise_blocks(ctx, p.tokens * plan.hidden / 4)), dim3(256), 0, use_stream(ctx),
+									reinterpret_cast<float*>(plan.dau), reinterpret_cast<float*>(plan.h), plan.dh, au, p.tokens, plan.hidden, up_offset());
 						});
 						MB200_COUNT_LAUNCH();
-						return check_cuda(ctx, cudaGetLastError(), "gated feed-forward: gate backward");
+						return check_cuda(ctx, status, "gated feed-forward: gate backward");
 					}
 				}
 				void forward(T *y, float beta, float *saved)
@@ -310,7 +362,7 @@ extern "C"
 			return;
 		const Plan plan(context, p, workspace.data, false, keep);
 		if (!check_workspace(context, who, workspace, plan.bytes) || !check_alignment(context, who, "x", x, plan.pack_x) || !check_alignment(context, who, "w1", w1, plan.pack_w1)
-				|| !check_alignment(context, who, "w2", w2, plan.pack_w2) || !check_alignment(context, who, "saved", saved, !plan.keeps))
+				|| !check_alignment(context, who, "w2", w2, plan.pack_w2) || !check_alignment(context, who, "saved", saved, !plan.keeps || plan.hidden != p.hidden))
 			return;
 		const struct { const char *name; const mlTensor_t &t; } inputs[] = { { "x", x }, { "w1", w1 }, { "w2", w2 } }, results[] = { { "y", y }, { "saved", saved }, { "workspace", workspace } };
 		for (int i = 0; i < 3; i++)
@@ -354,7 +406,7 @@ extern "C"
 		const Plan plan(context, p, workspace.data, true, kept);
 		if (!check_workspace(context, who, workspace, plan.bytes) || !check_alignment(context, who, "x", x, plan.pack_x) || !check_alignment(context, who, "dy", dy, plan.pack_x)
 				|| !check_alignment(context, who, "w1", w1, plan.pack_w1) || !check_alignment(context, who, "w2", w2, plan.pack_w2)
-				|| !check_alignment(context, who, "saved", saved, !plan.keeps))
+				|| !check_alignment(context, who, "saved", saved, !plan.keeps || plan.hidden != p.hidden))
 			return;
 		const struct { const char *name; const mlTensor_t &t; } inputs[] = { { "x", x }, { "w1", w1 }, { "w2", w2 }, { "saved", saved }, { "dy", dy } }, results[] = { { "dx", dx },
 				{ "dw1", dw1 }, { "dw2", dw2 }, { "workspace", workspace } };

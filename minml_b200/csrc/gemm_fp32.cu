@@ -1,8 +1,9 @@
 /*
  * gemm_fp32.cu -- fp32 matrix products that keep fp32 accuracy at any K, on the TF32 tensor cores.
  *
- * As in gemm_tc.cu, every element is split in shared memory into hi (x rounded to a TF32 number) and lo = x - hi, and hi hi + hi lo + lo hi
- * is accumulated; what is dropped is of relative size 2^-21.  But the tensor core cuts its sums instead of rounding them, measured
+ * Every element is split into hi, its upper 19 bits, which is what the tensor core reads of the fp32 tile as it lies in shared memory, and
+ * lo = x - hi rounded to TF32, which warps write to a tile of their own; hi hi + hi lo + lo hi is accumulated.  Dropped are lo lo, at most
+ * 2^-20 of the product and 2^-22 on average, and lo's rounding, 2^-21.  But the tensor core cuts its sums instead of rounding them, measured
  * 2e-8 of the sum for every 8 K indices and product, always toward zero: 3.7e-6 at K = 512 and 5.7e-5 at K = 8192, where an fp32 sum is off
  * by 4e-7 and 7e-7.  So an accumulator here takes one stage, 32 K indices (12 instructions, 2.3e-7), and the epilogue warps add it to sums that
  * they hold in registers, 64 columns a lane; four accumulators in tensor memory keep the tensor core ahead of them.
@@ -54,10 +55,11 @@ namespace mb200
 				uint32_t tmem_base;
 				int abort_flag;
 		};
-		__device__ __forceinline__ void split_tf32(uint32_t x, uint32_t &hi, uint32_t &lo)
+		/* What the upper 19 bits of x leave, rounded to TF32 (either way, so that the cut of the tensor core has nothing to cut). */
+		__device__ __forceinline__ uint32_t low_part(uint32_t x)
 		{
-			hi = (x + 0x1000u) & 0xFFFFE000u;
-			lo = __float_as_uint(__uint_as_float(x) - __uint_as_float(hi));
+			const float lo = __uint_as_float(x) - __uint_as_float(x & 0xFFFFE000u);
+			return (__float_as_uint(lo) + 0x1000u) & 0xFFFFE000u;
 		}
 
 		__global__ void __launch_bounds__(THREADS, 1) kernel_gemm_fp32(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Params p)
@@ -183,7 +185,7 @@ namespace mb200
 								break;
 							}
 							tcgen05_fence_after();
-							fence_proxy_async_smem(); // hi and lo were plain stores of the split warps
+							fence_proxy_async_smem(); // lo was written by plain stores of the split warps
 							const uint32_t d = tmem_base + b * BN;
 							const uint32_t hi = smem_base + s * STAGE_BYTES, lo = lo_base + (it % LO_STAGES) * STAGE_BYTES;
 							const uint64_t hi_a = describe(hi, p.a_mn), hi_b = describe(hi + OPERAND_BYTES, p.b_mn);
@@ -207,7 +209,7 @@ namespace mb200
 				__syncwarp();
 			}
 			else if (warp >= 2 + EPI_WARPS)
-			{ /* ------------------------------------------- split: x -> hi (in place) and lo */
+			{ /* ------------------------------------------- split: lo of every element */
 				const int t = threadIdx.x - (2 + EPI_WARPS) * 32;
 				uint32_t it = 0;
 				bool ok = true;
@@ -233,15 +235,7 @@ namespace mb200
 								x[i] = ld_shared_v4(hi + (t + (g + i) * SPLIT_WARPS * 32) * 16);
 #pragma unroll
 							for (int i = 0; i < GROUP; i++)
-							{
-								uint4 h, l;
-								split_tf32(x[i].x, h.x, l.x);
-								split_tf32(x[i].y, h.y, l.y);
-								split_tf32(x[i].z, h.z, l.z);
-								split_tf32(x[i].w, h.w, l.w);
-								st_shared_v4(hi + (t + (g + i) * SPLIT_WARPS * 32) * 16, h);
-								st_shared_v4(lo + (t + (g + i) * SPLIT_WARPS * 32) * 16, l);
-							}
+								st_shared_v4(lo + (t + (g + i) * SPLIT_WARPS * 32) * 16, make_uint4(low_part(x[i].x), low_part(x[i].y), low_part(x[i].z), low_part(x[i].w)));
 						}
 						fence_proxy_async_smem();
 						__syncwarp();
@@ -330,15 +324,28 @@ namespace mb200
 			}
 		}
 
+		/* Four destination elements a thread (pitch is a multiple of four). */
 		template<typename T>
 		__global__ void __launch_bounds__(256) kernel_pack_rows(T *__restrict__ dst, int pitch, long long padded_rows, const T *__restrict__ src, long long rows, int columns, int blocks)
 		{
-			for (long long r = blockIdx.x; r < padded_rows * blocks; r += gridDim.x)
+			struct alignas(4 * sizeof(T)) Four
 			{
-				const long long block = r / padded_rows, inside = r - block * padded_rows;
-				const T *from = src + (block * rows + inside) * columns;
-				for (int c = threadIdx.x; c < pitch; c += 256)
-					dst[r * pitch + c] = inside < rows && c < columns ? from[c] : from_float<T>(0.0f);
+					T v[4];
+			};
+			let_next_grid_start();
+			wait_for_previous_grid();
+			const int groups = pitch / 4;
+			const long long total = padded_rows * blocks * groups, stride = static_cast<long long>(gridDim.x) * 256;
+			for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < total; i += stride)
+			{
+				const long long r = i / groups, block = r / padded_rows, inside = r - block * padded_rows;
+				const int c = static_cast<int>(i - r * groups) * 4;
+				const T *from = src + (block * rows + inside) * columns + c;
+				Four out;
+#pragma unroll
+				for (int k = 0; k < 4; k++)
+					out.v[k] = inside < rows && c + k < columns ? from[k] : from_float<T>(0.0f);
+				*reinterpret_cast<Four*>(dst + r * pitch + c) = out;
 			}
 		}
 	}
@@ -346,15 +353,16 @@ namespace mb200
 	template<typename T>
 	bool pack_rows(mlContext_t ctx, T *dst, int pitch, long long padded_rows, const T *src, long long rows, int columns, int blocks)
 	{
-		const int grid = static_cast<int>(std::max<long long>(1, std::min<long long>(padded_rows * blocks, static_cast<long long>(get(ctx)->sm_count) * 8)));
-		kernel_pack_rows<T> <<<grid, 256, 0, use_stream(ctx)>>>(dst, pitch, padded_rows, src, rows, columns, blocks);
+		const long long threads = padded_rows * blocks * (pitch / 4);
+		const int grid = static_cast<int>(std::max<long long>(1, std::min<long long>((threads + 255) / 256, static_cast<long long>(get(ctx)->sm_count) * 16)));
+		const cudaError_t status = launch_overlapped(kernel_pack_rows<T>, dim3(grid), dim3(256), 0, use_stream(ctx), dst, pitch, padded_rows, src, rows, columns, blocks);
 		MB200_COUNT_LAUNCH();
-		return check_cuda(ctx, cudaGetLastError(), "pack_rows");
+		return check_cuda(ctx, status, "pack_rows");
 	}
 	template bool pack_rows<__half>(mlContext_t, __half*, int, long long, const __half*, long long, int, int);
 	template bool pack_rows<float>(mlContext_t, float*, int, long long, const float*, long long, int, int);
 
-	/* As pair_splits (gemm_pair.cu), with this kernel's figures: a K block of a tile 0.85 us. */
+	/* As pair_splits (gemm_pair.cu), with this kernel's figures: a K block of a tile 0.75 us. */
 	namespace
 	{
 		int float_splits(mlContext_t ctx, int M, int N, int K)
@@ -372,7 +380,7 @@ namespace mb200
 				const double partial_bytes = s == 1 ? 0.0 : 8.0 * s * M * N;
 				if (partial_bytes > 2.0 * (size_t(256) << 20))
 					break;
-				const double time = static_cast<double>((tiles * s + sms - 1) / sms) * (blocks * 0.85 + 1.5) + (s == 1 ? 0.0 : 4.0 + partial_bytes / 5.0e6);
+				const double time = static_cast<double>((tiles * s + sms - 1) / sms) * (blocks * 0.75 + 1.5) + (s == 1 ? 0.0 : 4.0 + partial_bytes / 5.0e6);
 				if (s == 1 || time < best_time)
 				{
 					best = s;
