@@ -32,12 +32,9 @@ def dtype_of(t):
 
 
 def shape_of(t_or_dims):
-    dims = list(t_or_dims.shape) if isinstance(t_or_dims, torch.Tensor) else list(t_or_dims)
-    s = mlShape_t()
-    s.rank = len(dims)
-    for i, d in enumerate(dims):
-        s.dim[i] = int(d)
-    return s
+    dims = t_or_dims.shape if isinstance(t_or_dims, torch.Tensor) else t_or_dims
+    rank = len(dims)
+    return mlShape_t.from_buffer_copy(_PACK_SHAPE(rank, *dims, *_FILL[rank]))
 
 
 def _check_device(t, ctx):
@@ -47,6 +44,7 @@ def _check_device(t, ctx):
         raise BackendError("tensor on cuda:%d passed to a context of cuda:%d" % (t.device.index, ctx.device_index))
 
 
+_PACK_SHAPE = struct.Struct("@7i").pack  # the layout of mlShape_t
 _EMPTY = mlTensor_t()  # null data, rank 0 (passed by value, so one instance serves every absent operand)
 _EMPTY.dtype = _abi.DTYPE_UNKNOWN
 _PACK = struct.Struct("@Qii6i").pack  # the layout of mlTensor_t; packing at once costs half of setting the fields one by one
@@ -370,9 +368,22 @@ def activationBackward(ctx, dy, y, dx, act="linear", alpha=1.0, beta=0.0):
 
 # ---------------------------------------------------------------------------------------------- training and serving of transformer blocks
 # (extensions: the reference has no counterpart; the C declarations in include/minml_b200.h say what each argument means)
+def _operand(t, ctx):
+    """desc for the functions below, which refuse what is not a dense tensor on the context's device instead of asserting."""
+    if t is None:
+        return _EMPTY
+    if t.get_device() != ctx.device_index:
+        raise BackendError("tensor on %s passed to a context of cuda:%d" % (t.device, ctx.device_index))
+    shape = t.shape
+    rank = len(shape)
+    if rank > 6 or not t.is_contiguous():
+        raise BackendError("a dense row-major tensor of at most 6 dimensions is needed, not %s with strides %s" % (tuple(shape), t.stride()))
+    return mlTensor_t.from_buffer_copy(_PACK(t.data_ptr(), _DTYPES.get(t.dtype, _abi.DTYPE_UNKNOWN), rank, *shape, *_FILL[rank]))
+
+
 def layernormForwardTraining(ctx, x, y, weights, bias, stats, ext=None):
     """layernormForward that also writes stats (fp32 [rows, 2]: mean and 1 / stddev of every row) for layernormBackward."""
-    lib.mb200_layernorm_forward(ctx.handle, desc(x, ctx), desc(ext, ctx), desc(weights, ctx), desc(bias, ctx), desc(y, ctx), desc(stats, ctx))
+    lib.mb200_layernorm_forward(ctx.handle, _operand(x, ctx), _operand(ext, ctx), _operand(weights, ctx), _operand(bias, ctx), _operand(y, ctx), _operand(stats, ctx))
     ctx.check()
 
 
@@ -383,8 +394,8 @@ def layernormBackwardGetWorkspaceSize(ctx, x_shape):
 
 def layernormBackward(ctx, x, dy, dx, weights, stats, dw=None, db=None, ext=None, beta_dx=0.0, beta_dw=0.0, workspace=None):
     """dx = gradient of x (and of ext) + beta_dx * dx; dw, db (fp32 or x's type) = gradients + beta_dw * old values, reduced in a fixed order."""
-    lib.mb200_layernorm_backward(ctx.handle, desc(x, ctx), desc(ext, ctx), desc(dy, ctx), desc(weights, ctx), desc(stats, ctx), beta_dx, desc(dx, ctx), beta_dw,
-                                 desc(dw, ctx), desc(db, ctx), desc(workspace, ctx))
+    lib.mb200_layernorm_backward(ctx.handle, _operand(x, ctx), _operand(ext, ctx), _operand(dy, ctx), _operand(weights, ctx), _operand(stats, ctx), beta_dx, _operand(dx, ctx), beta_dw,
+                                 _operand(dw, ctx), _operand(db, ctx), _operand(workspace, ctx))
     ctx.check()
 
 
@@ -410,14 +421,14 @@ def gatedFeedForwardGetWorkspaceSize(ctx, x_shape, w1_shape, dtype=torch.float16
 
 def gatedFeedForwardForward(ctx, x, w1, w2, y, gate="silu", beta=0.0, saved=None, workspace=None):
     """y = (act(x Wg^T) * (x Wu^T)) W2^T + beta * y, w1 = [Wg; Wu] of shape [2 hidden, embed], w2 of shape [embed, hidden]."""
-    lib.mb200_gated_feed_forward_forward(ctx.handle, desc(x, ctx), desc(w1, ctx), desc(w2, ctx), beta, desc(y, ctx), gate_code(gate), desc(saved, ctx), desc(workspace, ctx))
+    lib.mb200_gated_feed_forward_forward(ctx.handle, _operand(x, ctx), _operand(w1, ctx), _operand(w2, ctx), beta, _operand(y, ctx), gate_code(gate), _operand(saved, ctx), _operand(workspace, ctx))
     ctx.check()
 
 
 def gatedFeedForwardBackward(ctx, x, w1, w2, dy, dx=None, dw1=None, dw2=None, gate="silu", saved=None, beta_dx=0.0, beta_dw=0.0, workspace=None):
     """Gradients of gatedFeedForwardForward for dy; `saved` is the tensor given to the forward call, or None (then it is computed again)."""
-    lib.mb200_gated_feed_forward_backward(ctx.handle, desc(x, ctx), desc(w1, ctx), desc(w2, ctx), desc(saved, ctx), desc(dy, ctx), beta_dx, desc(dx, ctx), beta_dw,
-                                          desc(dw1, ctx), desc(dw2, ctx), gate_code(gate), desc(workspace, ctx))
+    lib.mb200_gated_feed_forward_backward(ctx.handle, _operand(x, ctx), _operand(w1, ctx), _operand(w2, ctx), _operand(saved, ctx), _operand(dy, ctx), beta_dx, _operand(dx, ctx), beta_dw,
+                                          _operand(dw1, ctx), _operand(dw2, ctx), gate_code(gate), _operand(workspace, ctx))
     ctx.check()
 
 
@@ -427,12 +438,12 @@ def softmaxCrossEntropyGetWorkspaceSize(ctx, x_shape, w_shape, dtype=torch.float
 
 def softmaxCrossEntropyForward(ctx, x, weights, targets, loss, lse=None, workspace=None):
     """loss[t] = log sum_v exp(x_t . w_v) - x_t . w_target (fp32), 0 for a target outside the vocabulary; lse[t] keeps the first term."""
-    lib.mb200_softmax_cross_entropy_forward(ctx.handle, desc(x, ctx), desc(weights, ctx), desc(targets, ctx), desc(loss, ctx), desc(lse, ctx), desc(workspace, ctx))
+    lib.mb200_softmax_cross_entropy_forward(ctx.handle, _operand(x, ctx), _operand(weights, ctx), _operand(targets, ctx), _operand(loss, ctx), _operand(lse, ctx), _operand(workspace, ctx))
     ctx.check()
 
 
 def softmaxCrossEntropyBackward(ctx, x, weights, targets, lse, dx=None, dw=None, alpha=1.0, row_weights=None, beta_dx=0.0, beta_dw=0.0, workspace=None):
     """Gradients of alpha * sum_t row_weights[t] * loss[t], each + beta times its old value."""
-    lib.mb200_softmax_cross_entropy_backward(ctx.handle, desc(x, ctx), desc(weights, ctx), desc(targets, ctx), desc(lse, ctx), alpha, desc(row_weights, ctx), beta_dx, desc(dx, ctx),
-                                             beta_dw, desc(dw, ctx), desc(workspace, ctx))
+    lib.mb200_softmax_cross_entropy_backward(ctx.handle, _operand(x, ctx), _operand(weights, ctx), _operand(targets, ctx), _operand(lse, ctx), alpha, _operand(row_weights, ctx), beta_dx, _operand(dx, ctx),
+                                             beta_dw, _operand(dw, ctx), _operand(workspace, ctx))
     ctx.check()

@@ -66,7 +66,7 @@ namespace mb200
 				// per epilogue warp: four 32 x 32 boxes of fp16 or two of fp32; GATED_RECOMPUTE: all six boxes of a tile
 				static constexpr int staging_bytes = EPI == GATED_RECOMPUTE ? 6 * 2048 : 8192;
 				static constexpr int stages = EPI == GATED_RECOMPUTE ? 4 : 5;
-				static constexpr bool moves_registers = EPI == GATED_RECOMPUTE || EPI == STATISTICS; // they hold 128 accumulators a thread
+				static constexpr bool moves_registers = EPI == GATED || EPI == GATED_RECOMPUTE || EPI == STATISTICS; // they hold 128 accumulators a thread
 				static constexpr int smem_bytes = stages * STAGE_BYTES + EPI_WARPS * staging_bytes + 1024;
 				static_assert(stages <= MAX_STAGES && smem_bytes <= 227 * 1024, "the configuration exceeds the SM");
 		};
@@ -134,12 +134,11 @@ namespace mb200
 			for (int k = 0; k < 4; k++)
 				st_shared_v4(box + lane * 64 + ((k ^ ((lane >> 1) & 3)) * 16), pack_half8(v + 8 * k));
 		}
-		__device__ __forceinline__ void write_float_box(uint32_t box, int lane, const float (&v)[32])
+		__device__ __forceinline__ void write_float_box(uint32_t box, int lane, const uint32_t (&v)[32])
 		{
 #pragma unroll
 			for (int k = 0; k < 8; k++)
-				st_shared_v4(box + lane * 128 + ((k ^ (lane & 7)) * 16),
-						make_uint4(__float_as_uint(v[4 * k]), __float_as_uint(v[4 * k + 1]), __float_as_uint(v[4 * k + 2]), __float_as_uint(v[4 * k + 3])));
+				st_shared_v4(box + lane * 128 + ((k ^ (lane & 7)) * 16), make_uint4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]));
 		}
 		__device__ __forceinline__ void load_chunk(uint32_t taddr, float (&v)[32])
 		{
@@ -478,23 +477,27 @@ namespace mb200
 						const int n0 = u.nt * (BN / 2) + half * 64;
 						// h of 64 columns: two boxes; two such pairs take turns, or, where a and u are kept, follow those through the same 8 KB
 						const uint32_t box = staging + (p.keep ? 0 : (boxes++ % 2) * 2 * HALF_BOX);
+						// this warp's accumulators into registers at once: the buffer goes back before the arithmetic
+						uint32_t a[2][32], b[2][32];
+#pragma unroll
+						for (int c = 0; c < 2; c++)
+						{
+							tmem_ld_32x32(taddr + half * 64 + c * 32, a[c]);
+							tmem_ld_32x32(taddr + BN / 2 + half * 64 + c * 32, b[c]);
+						}
+						tmem_wait_ld();
+						release();
 						uint32_t packed[2][16];
 #pragma unroll
 						for (int c = 0; c < 2; c++)
 						{
-							const int column = half * 64 + c * 32;
-							float a[32], b[32];
-							load_chunk(taddr + column, a);
-							load_chunk(taddr + BN / 2 + column, b);
-							if (c == 1)
-								release();
 							if (p.keep)
 							{
 								if (lane == 0)
 									bulk_wait_group_read<0>();
 								__syncwarp();
-								write_float_box(staging, lane, a);
-								write_float_box(staging + FLOAT_BOX, lane, b);
+								write_float_box(staging, lane, a[c]);
+								write_float_box(staging + FLOAT_BOX, lane, b[c]);
 								publish();
 								if (lane == 0 && row0 < p.M && n0 + c * 32 < p.N)
 								{
@@ -506,7 +509,8 @@ namespace mb200
 #pragma unroll
 							for (int j = 0; j < 32; j += 2)
 							{
-								const Pair h = pair_mul(gate_value<GATE>(Pair { a[j], a[j + 1] }), Pair { b[j], b[j + 1] });
+								const Pair h = pair_mul(gate_value<GATE>(Pair { __uint_as_float(a[c][j]), __uint_as_float(a[c][j + 1]) }),
+										Pair { __uint_as_float(b[c][j]), __uint_as_float(b[c][j + 1]) });
 								packed[c][j / 2] = pack_half2(h.x, h.y);
 							}
 						}
@@ -667,7 +671,11 @@ namespace mb200
 								bulk_wait_group_read<1>();
 							__syncwarp();
 							const uint32_t box = staging + (boxes++ % 2) * FLOAT_BOX;
-							write_float_box(box, lane, v);
+							uint32_t raw[32];
+#pragma unroll
+							for (int j = 0; j < 32; j++)
+								raw[j] = __float_as_uint(v[j]);
+							write_float_box(box, lane, raw);
 							publish();
 							if (lane == 0 && row0 < p.M)
 							{
@@ -895,22 +903,19 @@ namespace mb200
 #pragma unroll
 				for (int k = 0; k < VEC; k++)
 					v[k] = 0.0f;
-				for (int s = 0; s < splits; s++, src += range)
+#pragma unroll 6
+				for (int s = 0; s < splits; s++)
 				{
-					if (VEC % 4 == 0)
+					if (VEC == 4)
 					{
-#pragma unroll
-						for (int k = 0; k < VEC / 4; k++)
-						{
-							const float4 t = reinterpret_cast<const float4*>(src)[k];
-							v[4 * k] += t.x;
-							v[(4 * k + 1) % VEC] += t.y;
-							v[(4 * k + 2) % VEC] += t.z;
-							v[(4 * k + 3) % VEC] += t.w;
-						}
+						const float4 t = *reinterpret_cast<const float4*>(src + s * range);
+						v[0] += t.x;
+						v[1 % VEC] += t.y;
+						v[2 % VEC] += t.z;
+						v[3 % VEC] += t.w;
 					}
 					else
-						v[0] += src[0];
+						v[0] += src[s * range];
 				}
 				const float c = row_scale != nullptr ? row_scale[m] : 1.0f;
 				Out *dst = reinterpret_cast<Out*>(d + m * ldd + n);
@@ -931,8 +936,8 @@ namespace mb200
 	template<typename T>
 	bool finish_sums(mlContext_t ctx, T *d, int ldd, int M, int N, const float *sums, int pitch, int splits, float alpha, const float *alpha_device, const float *row_scale, float beta)
 	{
-		constexpr int VEC = 16 / sizeof(T);
-		const bool wide = N % VEC == 0 && ldd % VEC == 0 && pitch % 4 == 0 && aligned_to(d, 16) && aligned_to(sums, 16);
+		constexpr int VEC = 4;
+		const bool wide = N % VEC == 0 && ldd % VEC == 0 && pitch % 4 == 0 && aligned_to(d, VEC * sizeof(T)) && aligned_to(sums, 16);
 		const long long threads = static_cast<long long>(M) * (wide ? N / VEC : N);
 		const int blocks = static_cast<int>(std::max<long long>(1, std::min<long long>((threads + 255) / 256, static_cast<long long>(get(ctx)->sm_count) * 8)));
 		const cudaError_t status = launch_overlapped(wide ? kernel_finish_sums<T, VEC> : kernel_finish_sums<T, 1>, dim3(blocks), dim3(256), 0, use_stream(ctx), d, ldd, M, N, sums, pitch,
