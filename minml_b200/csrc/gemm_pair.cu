@@ -80,9 +80,7 @@ namespace mb200
 				PairResult result; // STORE
 				int direct; // STORE: element-wise stores, for results that TMA cannot address
 				int accumulate; // SUMS
-				int keep; // GATED: also write a and u
-				const float *au; // GATED_BACKWARD
-				int hidden;
+				float *kept; // a and u: written by GATED unless null, read by GATED_BACKWARD
 				const int *targets;
 				const float *row_weights, *lse;
 				int first, vocab;
@@ -117,6 +115,14 @@ namespace mb200
 			asm volatile(
 					"cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];"
 					:: "l"(reinterpret_cast<uint64_t>(map)), "r"(src), "r"(c0), "r"(c1) : "memory");
+		}
+
+		/* The kept a and u: for every 32 rows the a of all columns, then the u; of each, for every four columns, the rows' 16-byte pieces one after the other.
+		 * So a warp whose lanes are rows, as an epilogue's are, moves 512 contiguous bytes at a time.  This is the block of (row0, column), whose
+		 * columns are multiples of four; the u lie rows * columns floats behind the a. */
+		__device__ __forceinline__ float* kept_block(float *kept, const Params &p, int row0, int column)
+		{
+			return kept + static_cast<long long>(row0) * 2 * p.N + static_cast<long long>(column) * min(32, p.M - row0);
 		}
 
 		/* On the even CTA's barrier.  What it reports is that tensor memory has been read (ordered by tcgen05.fence), no memory write: a release at
@@ -475,8 +481,7 @@ namespace mb200
 					if (EPI == GATED)
 					{
 						const int n0 = u.nt * (BN / 2) + half * 64;
-						// h of 64 columns: two boxes; two such pairs take turns, or, where a and u are kept, follow those through the same 8 KB
-						const uint32_t box = staging + (p.keep ? 0 : (boxes++ % 2) * 2 * HALF_BOX);
+						const uint32_t box = staging + (boxes++ % 2) * 2 * HALF_BOX; // h of 64 columns: two boxes, two such pairs take turns
 						// this warp's accumulators into registers at once: the buffer goes back before the arithmetic
 						uint32_t a[2][32], b[2][32];
 #pragma unroll
@@ -491,20 +496,17 @@ namespace mb200
 #pragma unroll
 						for (int c = 0; c < 2; c++)
 						{
-							if (p.keep)
+							if (p.kept != nullptr && row_ok)
 							{
-								if (lane == 0)
-									bulk_wait_group_read<0>();
-								__syncwarp();
-								write_float_box(staging, lane, a[c]);
-								write_float_box(staging + FLOAT_BOX, lane, b[c]);
-								publish();
-								if (lane == 0 && row0 < p.M && n0 + c * 32 < p.N)
-								{
-									tma_store_2d(&map_e, staging, n0 + c * 32, row0);
-									tma_store_2d(&map_f, staging + FLOAT_BOX, n0 + c * 32, row0);
-									bulk_commit_group();
-								}
+								float *dst = kept_block(p.kept, p, row0, n0 + c * 32) + lane * 4;
+								const int rows = min(32, p.M - row0);
+#pragma unroll
+								for (int k = 0; k < 8; k++)
+									if (n0 + c * 32 + 4 * k < p.N)
+									{
+										*reinterpret_cast<uint4*>(dst + k * rows * 4) = make_uint4(a[c][4 * k], a[c][4 * k + 1], a[c][4 * k + 2], a[c][4 * k + 3]);
+										*reinterpret_cast<uint4*>(dst + k * rows * 4 + rows * p.N) = make_uint4(b[c][4 * k], b[c][4 * k + 1], b[c][4 * k + 2], b[c][4 * k + 3]);
+									}
 							}
 #pragma unroll
 							for (int j = 0; j < 32; j += 2)
@@ -515,12 +517,7 @@ namespace mb200
 							}
 						}
 						if (lane == 0)
-						{
-							if (p.keep)
-								bulk_wait_group_read<0>();
-							else
-								bulk_wait_group_read<1>();
-						}
+							bulk_wait_group_read<1>();
 						__syncwarp();
 #pragma unroll
 						for (int c = 0; c < 2; c++)
@@ -616,14 +613,14 @@ namespace mb200
 						if (EPI == GATED_BACKWARD)
 						{
 							float a[32], b[32];
-							const bool inside = row_ok && n < p.N; // hidden is a multiple of 8, so a chunk's 16-byte pieces are inside or outside
-							const float *src = p.au + static_cast<long long>(row) * 2 * p.hidden + n;
+							const int rows = min(32, p.M - row0);
+							const float *src = kept_block(p.kept, p, row0, n) + lane * 4;
 #pragma unroll
 							for (int k = 0; k < 8; k++)
 							{
-								const bool ok4 = inside && n + 4 * k < p.N;
-								const float4 ta = ok4 ? __ldg(reinterpret_cast<const float4*>(src) + k) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-								const float4 tb = ok4 ? __ldg(reinterpret_cast<const float4*>(src + p.hidden) + k) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+								const bool inside = row_ok && n + 4 * k < p.N;
+								const float4 ta = inside ? __ldg(reinterpret_cast<const float4*>(src + k * rows * 4)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+								const float4 tb = inside ? __ldg(reinterpret_cast<const float4*>(src + k * rows * 4 + rows * p.N)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 								a[4 * k] = ta.x, a[4 * k + 1] = ta.y, a[4 * k + 2] = ta.z, a[4 * k + 3] = ta.w;
 								b[4 * k] = tb.x, b[4 * k + 1] = tb.y, b[4 * k + 2] = tb.z, b[4 * k + 3] = tb.w;
 							}
@@ -848,13 +845,6 @@ namespace mb200
 			const uint32_t box[2] = { 32, 32 };
 			return encode_tensor_map(ctx, map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, d, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_64B);
 		}
-		bool map_floats(mlContext_t ctx, CUtensorMap *map, const void *d, int ld, int rows, int columns)
-		{
-			const uint64_t dims[2] = { static_cast<uint64_t>(columns), static_cast<uint64_t>(rows) };
-			const uint64_t strides[1] = { static_cast<uint64_t>(ld) * 4 };
-			const uint32_t box[2] = { 32, 32 };
-			return encode_tensor_map(ctx, map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, d, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
-		}
 		/* Operand maps and tile counts; the result maps are filled with a copy where an epilogue has no use for them. */
 		bool prepare(mlContext_t ctx, Maps &maps, Params &p, int M, int N, int K, const PairOperand &a, const PairOperand &b, int b_rows, int tile_columns, int splits)
 		{
@@ -1021,30 +1011,27 @@ namespace mb200
 		return launch<SUMS, 0>(ctx, maps, p);
 	}
 
-	bool pair_gated(mlContext_t ctx, int tokens, int embed, int hidden, const PairOperand &x, const PairOperand &w1, int gate, __half *h, int ldh, float *au)
+	bool pair_gated(mlContext_t ctx, int tokens, int embed, int hidden, const PairOperand &x, const PairOperand &w1, int gate, __half *h, int ldh, float *kept)
 	{
 		Maps maps;
 		Params p;
 		if (!prepare(ctx, maps, p, tokens, hidden, embed, x, w1, 2 * hidden, BN / 2, 1) || !map_halves(ctx, &maps.d, h, ldh, tokens, hidden))
 			return false;
 		p.up_row = hidden;
-		p.keep = au != nullptr;
-		if (au != nullptr && (!map_floats(ctx, &maps.e, au, 2 * hidden, tokens, hidden) || !map_floats(ctx, &maps.f, au + hidden, 2 * hidden, tokens, hidden)))
-			return false;
+		p.kept = kept;
 		return with_gate(gate, [&](auto g)
 		{
 			return launch<GATED, decltype(g)::value>(ctx, maps, p);
 		});
 	}
-	bool pair_gated_backward(mlContext_t ctx, int tokens, int embed, int hidden, const PairOperand &dy, const PairOperand &w2, int gate, const float *au, __half *dau, __half *h)
+	bool pair_gated_backward(mlContext_t ctx, int tokens, int embed, int hidden, const PairOperand &dy, const PairOperand &w2, int gate, const float *kept, __half *dau, __half *h)
 	{
 		Maps maps;
 		Params p;
 		if (!prepare(ctx, maps, p, tokens, hidden, embed, dy, w2, hidden, BN, 1) || !map_halves(ctx, &maps.d, dau, 2 * hidden, tokens, hidden)
 				|| !map_halves(ctx, &maps.e, dau + hidden, 2 * hidden, tokens, hidden) || !map_halves(ctx, &maps.f, h, hidden, tokens, hidden))
 			return false;
-		p.au = au;
-		p.hidden = hidden;
+		p.kept = const_cast<float*>(kept);
 		return with_gate(gate, [&](auto g)
 		{
 			return launch<GATED_BACKWARD, decltype(g)::value>(ctx, maps, p);

@@ -39,13 +39,13 @@ namespace mb200
 	bool finish_sums(mlContext_t ctx, T *d, int ldd, int M, int N, const float *sums, int pitch, int splits, float alpha, const float *alpha_device, const float *row_scale, float beta);
 
 	/* h = act(a) u with a = x Wg^T, u = x Wu^T, w1 = [Wg; Wu] (2 hidden rows).  h [tokens, hidden], pitch ldh (a multiple of 8 elements, 16-byte
-	 * aligned).  au: null, or fp32 [tokens, 2 hidden] that receives a and u (hidden a multiple of 4). */
-	bool pair_gated(mlContext_t ctx, int tokens, int embed, int hidden, const PairOperand &x, const PairOperand &w1, int gate, __half *h, int ldh, float *au);
-	/* From dh = dy W2 and the kept au: dau = [dh u act'(a), dh act(a)] fp16 [tokens, 2 hidden], h = act(a) u fp16 [tokens, hidden]; hidden a
+	 * aligned).  kept: null, or 2 tokens hidden floats that receive a and u, in an order of this kernel's own (hidden a multiple of 4). */
+	bool pair_gated(mlContext_t ctx, int tokens, int embed, int hidden, const PairOperand &x, const PairOperand &w1, int gate, __half *h, int ldh, float *kept);
+	/* From dh = dy W2 and what pair_gated kept: dau = [dh u act'(a), dh act(a)] fp16 [tokens, 2 hidden], h = act(a) u fp16 [tokens, hidden]; hidden a
 	 * multiple of 8. */
-	bool pair_gated_backward(mlContext_t ctx, int tokens, int embed, int hidden, const PairOperand &dy, const PairOperand &w2, int gate, const float *au, __half *dau, __half *h);
+	bool pair_gated_backward(mlContext_t ctx, int tokens, int embed, int hidden, const PairOperand &dy, const PairOperand &w2, int gate, const float *kept, __half *dau, __half *h);
 
-	/* The same without a kept au: a and u are made again, in the same tiles as dh.  dy [tokens, embed] and w2 stored [embed, hidden] (mn). */
+	/* The same with nothing kept: a and u are made again, in the same tiles as dh.  dy [tokens, embed] and w2 stored [embed, hidden] (mn). */
 	bool pair_gated_recompute(mlContext_t ctx, int tokens, int embed, int hidden, const PairOperand &x, const PairOperand &w1, const PairOperand &dy, const PairOperand &w2, int gate, __half *dau,
 			__half *h);
 
