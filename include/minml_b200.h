@@ -295,7 +295,8 @@ void mb200_convolution_forward_noalloc(mlContext_t context, mlDataType_t dtype, 
  * is a matrix of boards * h * w rows).  A descriptor with null data and rank 0 stands for an absent optional operand.  Scratch memory
  * is the caller's: mb200_*_get_workspace_size tells how much, `workspace` is a descriptor of at least that many bytes, 16-byte aligned,
  * whose contents need not survive between calls; calls that may overlap on the GPU (two contexts, two replayed graphs) need one each.
- * No call allocates or synchronises, so each may be captured into a CUDA graph.  Results do not depend on timing (no atomics in sums):
+ * fp16 and fp32 matrices whose row length is a multiple of 16 bytes must be 16-byte aligned (where they are operands of a product), others
+ * are copied to padded rows in the workspace first.  No call allocates or synchronises, so each may be captured into a CUDA graph.  Results do not depend on timing (no atomics in sums):
  * the same call gives the same bits. */
 
 /* Layer normalisation that keeps what its backward pass needs: y as cuda_layernorm_forward, stats [rows, 2] fp32 = (mean, 1 / stddev) of
@@ -309,7 +310,8 @@ void mb200_layernorm_backward(mlContext_t context, const mlTensor_t x, const mlT
 
 /* Gated feed-forward block: y = (act(x Wg^T) * (x Wu^T)) W2^T + beta * y with W1 = [Wg; Wu], a [2 hidden, embed] matrix (gate rows first), and
  * W2 [embed, hidden].  `gate` names act.  `saved` (optional, fp32 [tokens, 2 hidden]) is where the forward pass may leave what its backward
- * pass reads instead of computing it again; its contents are the library's own. */
+ * pass reads instead of computing it again; its contents are the library's own.  Where making it again is cheaper (fp16 with embed up to
+ * 1024 or hidden no multiple of 8) it is left as it was: such a caller need not provide it. */
 #define MB200_GATE_SIGMOID 0
 #define MB200_GATE_RELU 1
 #define MB200_GATE_SILU 2

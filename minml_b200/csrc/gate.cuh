@@ -64,9 +64,11 @@ namespace mb200
 	{
 		if (GATE == MB200_GATE_SILU || GATE == MB200_GATE_SIGMOID)
 		{
-			const Pair s = sigmoid_fast(g), rest = pair_fma(s, Pair { -1.0f, -1.0f }, Pair { 1.0f, 1.0f }); // 1 - s
-			// (a NaN has passed sigmoid_fast as if it were large)
-			value = GATE == MB200_GATE_SIGMOID ? Pair { g.x == g.x ? s.x : g.x, g.y == g.y ? s.y : g.y } : pair_mul(g, s);
+			Pair s = sigmoid_fast(g);
+			if (GATE == MB200_GATE_SIGMOID)
+				s = Pair { g.x == g.x ? s.x : g.x, g.y == g.y ? s.y : g.y }; // (a NaN has passed sigmoid_fast as if it were large)
+			const Pair rest = pair_fma(s, pair_of(-1.0f), pair_of(1.0f)); // 1 - s
+			value = GATE == MB200_GATE_SIGMOID ? s : pair_mul(g, s);
 			derivative = GATE == MB200_GATE_SIGMOID ? pair_mul(s, rest) : pair_fma(value, rest, s); // silu: s + g s (1 - s)
 		}
 		else

@@ -10,6 +10,7 @@ would drive:
   Add                     src/layers/Add.cpp:50-60
   LayerNormalization      src/layers/LayerNormalization.cpp:86-95
   MultiHeadAttention      src/layers/MultiHeadAttention.cpp:92-101
+  GatedFeedForward, SoftmaxCrossEntropy, LayerNormalization's training half: extensions without a counterpart in the reference
   ResNetTrunk / HybridBlock   the node loop of Graph::predict (src/graph/Graph.cpp:241-248) over the benchmark topologies,
                           after the FoldAdd pass (src/graph/graph_optimizers.cpp:186-218): the skip connection rides in
                           the second convolution of a block as its `ext` input.
@@ -170,6 +171,55 @@ class LayerNormalization:
 
     def forward(self, inputs, output, workspace=None):
         B.layernormForward(self.ctx, inputs[0], output, self.gamma, self.beta, inputs[1] if len(inputs) > 1 else None)
+
+    # training: stats (fp32 [rows, 2]) is the caller's, so that one layer can be used for several batches in flight
+    def forward_training(self, inputs, output, stats):
+        B.layernormForwardTraining(self.ctx, inputs[0], output, self.gamma, self.beta, stats, inputs[1] if len(inputs) > 1 else None)
+
+    def backward_workspace_bytes(self, in_shape):
+        return B.layernormBackwardGetWorkspaceSize(self.ctx, in_shape)
+
+    def backward(self, inputs, stats, gradient_next, gradient_prev, gamma_update, beta_update, workspace, beta_prev=0.0, beta_update_factor=0.0):
+        """gradient_prev = gradient of inputs[0] (and of the summand inputs[1]) + beta_prev * gradient_prev."""
+        B.layernormBackward(self.ctx, inputs[0], gradient_next, gradient_prev, self.gamma, stats, gamma_update, beta_update, ext=inputs[1] if len(inputs) > 1 else None,
+                            beta_dx=beta_prev, beta_dw=beta_update_factor, workspace=workspace.buffer)
+
+
+class GatedFeedForward:
+    """y = (act(x Wg^T) * (x Wu^T)) W2^T (+ y), w1 = [Wg; Wu] of shape [2 hidden, embed], w2 of shape [embed, hidden] (numpy fp32)."""
+
+    def __init__(self, ctx, w1, w2, gate="silu", dtype=torch.float16):
+        self.ctx, self.gate, self.dtype = ctx, gate, dtype
+        self.w1, self.w2 = _dev(ctx, w1, dtype), _dev(ctx, w2, dtype)
+
+    def workspace_bytes(self, in_shape, training=False, saved=True):
+        return B.gatedFeedForwardGetWorkspaceSize(self.ctx, in_shape, self.w1.shape, self.dtype, training, saved)
+
+    def forward(self, inputs, output, workspace, saved=None, beta=0.0):
+        """beta = 1: added to what `output` holds (the residual sum)."""
+        B.gatedFeedForwardForward(self.ctx, inputs[0], self.w1, self.w2, output, self.gate, beta=beta, saved=saved, workspace=workspace.buffer)
+
+    def backward(self, inputs, gradient_next, gradient_prev, w1_update, w2_update, workspace, saved=None, beta_prev=0.0, beta_update_factor=0.0):
+        B.gatedFeedForwardBackward(self.ctx, inputs[0], self.w1, self.w2, gradient_next, gradient_prev, w1_update, w2_update, self.gate, saved=saved, beta_dx=beta_prev,
+                                   beta_dw=beta_update_factor, workspace=workspace.buffer)
+
+
+class SoftmaxCrossEntropy:
+    """A bias-free output layer [vocabulary, embed] (numpy fp32) together with the loss of its softmax: the logits are never kept."""
+
+    def __init__(self, ctx, weights, dtype=torch.float16):
+        self.ctx, self.dtype = ctx, dtype
+        self.weights = _dev(ctx, weights, dtype)
+
+    def workspace_bytes(self, in_shape, training=False):
+        return B.softmaxCrossEntropyGetWorkspaceSize(self.ctx, in_shape, self.weights.shape, self.dtype, training)
+
+    def forward(self, inputs, targets, loss, workspace, lse=None):
+        B.softmaxCrossEntropyForward(self.ctx, inputs[0], self.weights, targets, loss, lse, workspace.buffer)
+
+    def backward(self, inputs, targets, lse, gradient_prev, weights_update, workspace, alpha=1.0, row_weights=None, beta_prev=0.0, beta_update_factor=0.0):
+        B.softmaxCrossEntropyBackward(self.ctx, inputs[0], self.weights, targets, lse, gradient_prev, weights_update, alpha, row_weights=row_weights, beta_dx=beta_prev,
+                                      beta_dw=beta_update_factor, workspace=workspace.buffer)
 
 
 class MultiHeadAttention:
