@@ -32,10 +32,11 @@ namespace mb200
 		constexpr int BM = 128, BN = 128, BK = 32;
 		constexpr int OPERAND_BYTES = 128 * 128;
 		constexpr int STAGE_BYTES = 2 * OPERAND_BYTES;
-		constexpr int STAGES = 5, LO_STAGES = 2, BUFFERS = 4;
+		constexpr int STAGES = 4, LO_STAGES = 2, BUFFERS = 4;
 		constexpr int EPI_WARPS = 8, SPLIT_WARPS = 4;
 		constexpr int THREADS = (2 + EPI_WARPS + SPLIT_WARPS) * 32;
-		constexpr int SMEM_BYTES = (STAGES + LO_STAGES) * STAGE_BYTES + 1024;
+		constexpr int BOX_BYTES = 32 * 128; // per epilogue warp: 32 x 32 results
+		constexpr int SMEM_BYTES = (STAGES + LO_STAGES) * STAGE_BYTES + EPI_WARPS * BOX_BYTES + 1024;
 
 		struct Params
 		{
@@ -281,30 +282,31 @@ namespace mb200
 							v[32 + j] += __uint_as_float(r1[j]);
 						}
 					}
-					const int row = u.m0 + q * 32 + lane, n0 = u.n0 + half * (BN / 2);
-					if (!ok || row >= p.M)
-						continue;
-					float *dst = p.d + (static_cast<long long>(u.split) * p.M + row) * p.ldd + n0;
-					if (n0 + BN / 2 <= p.N && p.ldd % 4 == 0 && aligned_to_16(p.d))
-					{
+					if (!ok)
+						break;
+					// a lane holds 64 columns of one row; through shared memory, so that a store instruction covers 128 bytes of one row
+					const int row0 = u.m0 + q * 32, rows = min(32, p.M - row0);
+					const uint32_t box = lo_base + LO_STAGES * STAGE_BYTES + (warp - 2) * BOX_BYTES;
 #pragma unroll
-						for (int j = 0; j < BN / 2; j += 4)
+					for (int c = 0; c < 2; c++)
+					{
+						const int n = u.n0 + half * (BN / 2) + c * 32 + lane;
+#pragma unroll
+						for (int k = 0; k < 8; k++)
+							st_shared_v4(box + lane * 128 + ((k ^ (lane & 7)) * 16), make_uint4(__float_as_uint(v[c * 32 + 4 * k]), __float_as_uint(v[c * 32 + 4 * k + 1]),
+									__float_as_uint(v[c * 32 + 4 * k + 2]), __float_as_uint(v[c * 32 + 4 * k + 3])));
+						__syncwarp();
+						if (n < p.N)
 						{
-							float4 t = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-							if (p.beta != 0.0f)
+							float *dst = p.d + (static_cast<long long>(u.split) * p.M + row0) * p.ldd + n;
+#pragma unroll 8
+							for (int r = 0; r < rows; r++, dst += p.ldd)
 							{
-								const float4 old = *reinterpret_cast<const float4*>(dst + j);
-								t = make_float4(t.x + p.beta * old.x, t.y + p.beta * old.y, t.z + p.beta * old.z, t.w + p.beta * old.w);
+								const float x = ld_shared_f32(box + r * 128 + (((lane / 4) ^ (r & 7)) * 16) + lane % 4 * 4);
+								*dst = p.beta != 0.0f ? x + p.beta * *dst : x;
 							}
-							*reinterpret_cast<float4*>(dst + j) = t;
 						}
-					}
-					else
-					{
-#pragma unroll
-						for (int j = 0; j < BN / 2; j++)
-							if (n0 + j < p.N)
-								dst[j] = p.beta != 0.0f ? v[j] + p.beta * dst[j] : v[j];
+						__syncwarp();
 					}
 				}
 			}

@@ -716,11 +716,18 @@ namespace mb200
 								}
 							}
 							if (p.direct)
-							{
-#pragma unroll
-								for (int j = 0; j < 32; j++)
-									if (row_ok && n + j < p.N)
-										dst[j] = __float2half_rn(v[j]);
+							{ // rows that TMA cannot address: through a box, so that a store instruction covers 64 bytes of one row instead of 2 bytes of 32
+								write_half_box(staging, lane, v);
+								__syncwarp();
+								const int rows = min(32, p.M - row0);
+								if (n + lane < p.N)
+									for (int r = 0; r < rows; r++)
+									{
+										uint16_t bits;
+										asm volatile("ld.shared.u16 %0, [%1];" : "=h"(bits) : "r"(staging + r * 64 + (((lane / 8) ^ ((r >> 1) & 3)) * 16) + lane % 8 * 2) : "memory");
+										*reinterpret_cast<uint16_t*>(p.result.d + static_cast<long long>(row0 + r) * p.result.ldd + n + lane) = bits;
+									}
+								__syncwarp();
 								continue;
 							}
 						}
