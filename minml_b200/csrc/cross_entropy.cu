@@ -131,16 +131,17 @@ namespace mb200
 		}
 
 		/* z becomes alpha c_t (exp(z - lse) - [target]) for one piece, four columns a thread; rows that take no part are zero */
-		__global__ void __launch_bounds__(256) kernel_piece_gradient(float *__restrict__ z, int pitch, const float *__restrict__ lse, Rows rows, long long tokens, int first, int width,
-				float alpha)
+		__global__ void __launch_bounds__(256) kernel_piece_gradient(float *__restrict__ z, int pitch, const float *__restrict__ lse, Rows rows, const GridWalk walk, int first, float alpha)
 		{
 			wait_for_previous_grid();
-			const int groups = (width + 3) / 4;
-			const long long total = tokens * groups, stride = static_cast<long long>(gridDim.x) * 256;
-			for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < total; i += stride)
+			const long long stride = static_cast<long long>(gridDim.x) * 256;
+			for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < walk.total; i += stride)
 			{
-				const long long t = i / groups;
-				const int c = static_cast<int>(i - t * groups) * 4, target = rows.targets[t] - first - c;
+				long long t;
+				int c;
+				walk.place(i, t, c);
+				c *= 4;
+				const int target = rows.targets[t] - first - c;
 				const float weight = rows.weight(t), l = lse[t], factor = alpha * weight;
 				float4 *at = reinterpret_cast<float4*>(z + t * pitch + c);
 				float4 v = *at;
@@ -438,7 +439,7 @@ namespace mb200
 					if (!float_product(ctx, tokens, width, D, FloatOperand { o.x, ld, false }, FloatOperand { w, ld, false }, plan.z, plan.pitch, 0.0f, plan.partials))
 						return;
 					const cudaError_t status = launch_overlapped(kernel_piece_gradient, dim3(elementwise_blocks(ctx, q.tokens * ((width + 3) / 4))), dim3(256), 0, stream, plan.z, plan.pitch, lse,
-							rows, q.tokens, first, width, alpha);
+							rows, GridWalk(q.tokens, (width + 3) / 4), first, alpha);
 					MB200_COUNT_LAUNCH();
 					if (!check_cuda(ctx, status, "mb200_softmax_cross_entropy_backward: probabilities"))
 						return;

@@ -47,16 +47,17 @@ namespace mb200
 			}
 		}
 		template<int GATE>
-		__global__ void __launch_bounds__(256) kernel_gate(float *__restrict__ h, const float *__restrict__ au, long long tokens, int hidden, int up)
+		__global__ void __launch_bounds__(256) kernel_gate(float *__restrict__ h, const float *__restrict__ au, const GridWalk walk, int hidden, int up)
 		{
 			let_next_grid_start();
 			wait_for_previous_grid();
-			const int groups = hidden / 4;
-			const long long total = tokens * groups, stride = static_cast<long long>(gridDim.x) * 256;
-			for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < total; i += stride)
+			const long long stride = static_cast<long long>(gridDim.x) * 256;
+			for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < walk.total; i += stride)
 			{
-				const long long t = i / groups;
-				const int c = static_cast<int>(i - t * groups) * 4;
+				long long t;
+				int c;
+				walk.place(i, t, c);
+				c *= 4;
 				Four a, u;
 				load_pre_activations(a, u, au, t, c, up);
 #pragma unroll
@@ -67,17 +68,18 @@ namespace mb200
 		}
 		/* [da du] and h from dh [tokens, hidden] and the pre-activations */
 		template<int GATE>
-		__global__ void __launch_bounds__(256) kernel_gate_backward(float *__restrict__ dau, float *__restrict__ h, const float *__restrict__ dh, const float *__restrict__ au, long long tokens,
-				int hidden, int up)
+		__global__ void __launch_bounds__(256) kernel_gate_backward(float *__restrict__ dau, float *__restrict__ h, const float *__restrict__ dh, const float *__restrict__ au,
+				const GridWalk walk, int hidden, int up)
 		{
 			let_next_grid_start();
 			wait_for_previous_grid();
-			const int groups = hidden / 4;
-			const long long total = tokens * groups, stride = static_cast<long long>(gridDim.x) * 256;
-			for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < total; i += stride)
+			const long long stride = static_cast<long long>(gridDim.x) * 256;
+			for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < walk.total; i += stride)
 			{
-				const long long t = i / groups;
-				const int c = static_cast<int>(i - t * groups) * 4;
+				long long t;
+				int c;
+				walk.place(i, t, c);
+				c *= 4;
 				Four a, u, d = *reinterpret_cast<const Four*>(dh + t * hidden + c);
 				load_pre_activations(a, u, au, t, c, up);
 #pragma unroll
@@ -215,7 +217,7 @@ namespace mb200
 						with_gate(p.gate, [&](auto gate)
 						{
 							status = launch_overlapped(kernel_gate<decltype(gate)::value>, dim3(elementwise_blocks(ctx, p.tokens * plan.hidden / 4)), dim3(256), 0, use_stream(ctx),
-									reinterpret_cast<float*>(plan.h), au, p.tokens, plan.hidden, up);
+									reinterpret_cast<float*>(plan.h), au, GridWalk(p.tokens, plan.hidden / 4), plan.hidden, up);
 						});
 						MB200_COUNT_LAUNCH();
 						return check_cuda(ctx, status, "gated feed-forward: gate");
@@ -242,7 +244,8 @@ namespace mb200
 						with_gate(p.gate, [&](auto gate)
 						{
 							status = launch_overlapped(kernel_gate_backward<decltype(gate)::value>, dim3(elementwise_blocks(ctx, p.tokens * plan.hidden / 4)), dim3(256), 0, use_stream(ctx),
-									reinterpret_cast<float*>(plan.dau), reinterpret_cast<float*>(plan.h), plan.dh, au, p.tokens, plan.hidden, up_offset());
+									reinterpret_cast<float*>(plan.dau), reinterpret_cast<float*>(plan.h), plan.dh, au, GridWalk(p.tokens, plan.hidden / 4), plan.hidden,
+									up_offset());
 						});
 						MB200_COUNT_LAUNCH();
 						return check_cuda(ctx, status, "gated feed-forward: gate backward");

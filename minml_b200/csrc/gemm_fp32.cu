@@ -328,7 +328,7 @@ namespace mb200
 
 		/* Four destination elements a thread (pitch is a multiple of four). */
 		template<typename T>
-		__global__ void __launch_bounds__(256) kernel_pack_rows(T *__restrict__ dst, int pitch, long long padded_rows, const T *__restrict__ src, long long rows, int columns, int blocks)
+		__global__ void __launch_bounds__(256) kernel_pack_rows(T *__restrict__ dst, int pitch, long long padded_rows, const T *__restrict__ src, long long rows, int columns, const GridWalk walk)
 		{
 			struct alignas(4 * sizeof(T)) Four
 			{
@@ -336,12 +336,16 @@ namespace mb200
 			};
 			let_next_grid_start();
 			wait_for_previous_grid();
-			const int groups = pitch / 4;
-			const long long total = padded_rows * blocks * groups, stride = static_cast<long long>(gridDim.x) * 256;
-			for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < total; i += stride)
+			const long long stride = static_cast<long long>(gridDim.x) * 256;
+			for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < walk.total; i += stride)
 			{
-				const long long r = i / groups, block = r / padded_rows, inside = r - block * padded_rows;
-				const int c = static_cast<int>(i - r * groups) * 4;
+				long long r;
+				int c;
+				walk.place(i, r, c);
+				c *= 4;
+				long long block = 0, inside = r;
+				for (; inside >= padded_rows; inside -= padded_rows) // at most two blocks
+					block++;
 				const T *from = src + (block * rows + inside) * columns + c;
 				Four out;
 #pragma unroll
@@ -357,7 +361,8 @@ namespace mb200
 	{
 		const long long threads = padded_rows * blocks * (pitch / 4);
 		const int grid = static_cast<int>(std::max<long long>(1, std::min<long long>((threads + 255) / 256, static_cast<long long>(get(ctx)->sm_count) * 16)));
-		const cudaError_t status = launch_overlapped(kernel_pack_rows<T>, dim3(grid), dim3(256), 0, use_stream(ctx), dst, pitch, padded_rows, src, rows, columns, blocks);
+		const cudaError_t status = launch_overlapped(kernel_pack_rows<T>, dim3(grid), dim3(256), 0, use_stream(ctx), dst, pitch, padded_rows, src, rows, columns,
+				GridWalk(padded_rows * blocks, pitch / 4));
 		MB200_COUNT_LAUNCH();
 		return check_cuda(ctx, status, "pack_rows");
 	}

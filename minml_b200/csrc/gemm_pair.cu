@@ -879,7 +879,7 @@ namespace mb200
 
 		/* One thread a group of VEC columns: the K ranges' sums in order, the factors, one rounding. */
 		template<typename T, int VEC>
-		__global__ void __launch_bounds__(256) kernel_finish_sums(T *d, int ldd, int M, int N, const float *__restrict__ sums, int pitch, int splits, float alpha,
+		__global__ void __launch_bounds__(256) kernel_finish_sums(T *d, int ldd, int M, const GridWalk walk, const float *__restrict__ sums, int pitch, int splits, float alpha,
 				const float *__restrict__ alpha_device, const float *__restrict__ row_scale, float beta)
 		{
 			struct alignas(sizeof(T) * VEC) Out
@@ -889,12 +889,13 @@ namespace mb200
 			wait_for_previous_grid();
 			if (alpha_device != nullptr)
 				alpha *= *alpha_device;
-			const int groups = (N + VEC - 1) / VEC;
-			const long long total = static_cast<long long>(M) * groups, stride = static_cast<long long>(gridDim.x) * 256, range = static_cast<long long>(M) * pitch;
-			for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < total; i += stride)
+			const long long stride = static_cast<long long>(gridDim.x) * 256, range = static_cast<long long>(M) * pitch;
+			for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < walk.total; i += stride)
 			{
-				const long long m = i / groups;
-				const int n = static_cast<int>(i - m * groups) * VEC;
+				long long m;
+				int n;
+				walk.place(i, m, n);
+				n *= VEC;
 				const float *src = sums + m * pitch + n;
 				float v[VEC];
 #pragma unroll
@@ -937,7 +938,7 @@ namespace mb200
 		const bool wide = N % VEC == 0 && ldd % VEC == 0 && pitch % 4 == 0 && aligned_to(d, VEC * sizeof(T)) && aligned_to(sums, 16);
 		const long long threads = static_cast<long long>(M) * (wide ? N / VEC : N);
 		const int blocks = static_cast<int>(std::max<long long>(1, std::min<long long>((threads + 255) / 256, static_cast<long long>(get(ctx)->sm_count) * 8)));
-		const cudaError_t status = launch_overlapped(wide ? kernel_finish_sums<T, VEC> : kernel_finish_sums<T, 1>, dim3(blocks), dim3(256), 0, use_stream(ctx), d, ldd, M, N, sums, pitch,
+		const cudaError_t status = launch_overlapped(wide ? kernel_finish_sums<T, VEC> : kernel_finish_sums<T, 1>, dim3(blocks), dim3(256), 0, use_stream(ctx), d, ldd, M, GridWalk(M, wide ? N / VEC : N), sums, pitch,
 				splits, alpha, alpha_device, row_scale, beta);
 		MB200_COUNT_LAUNCH();
 		return check_cuda(ctx, status, "finish_sums");

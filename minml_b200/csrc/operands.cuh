@@ -134,6 +134,37 @@ namespace mb200
 		mlTensor_t t = { };
 		return t;
 	}
+	/* Walks a grid over rows x groups: a 64-bit division by a run-time number is dozens of instructions, so up to 2^31 places go by FastDiv. */
+	struct GridWalk
+	{
+			long long total;
+			long long groups;
+			FastDiv by_groups;
+			int small;
+			GridWalk() = default;
+			GridWalk(long long rows, long long groups_of_row) :
+					total(rows * groups_of_row),
+					groups(groups_of_row),
+					by_groups(static_cast<uint32_t>(groups_of_row <= 0x7FFFFFFFll ? groups_of_row : 1)),
+					small(total <= 0x7FFFFFFFll)
+			{
+			}
+			__device__ __forceinline__ void place(long long i, long long &row, int &group) const
+			{
+				if (small)
+				{
+					uint32_t q, r;
+					by_groups.divmod(static_cast<uint32_t>(i), q, r);
+					row = q;
+					group = static_cast<int>(r);
+				}
+				else
+				{
+					row = i / groups;
+					group = static_cast<int>(i - row * groups);
+				}
+			}
+	};
 	/* Launch whose grid may start before the grid ahead of it in the stream has finished; the kernel calls griddepcontrol.wait
 	 * (wait_for_previous_grid) before it touches anything that grid wrote. */
 	template<typename ... KArgs, typename ... Args>
