@@ -401,21 +401,38 @@ namespace mb200
 				cluster_sync();
 				const int row = threadIdx.x, n = g0 * GROUP + row;
 				if (row < 128 && row < (g1 - g0) * GROUP && n < p.N)
+				{
+					uint32_t from[MAX_CLUSTER]; // this row's sums of token 0 in every CTA
+#pragma unroll
+					for (int k = 0; k < MAX_CLUSTER; k++)
+						from[k] = map_to_cta(smem_base + row * 4, min(k, p.cluster - 1));
+#pragma unroll 2
 					for (int t = rank; t < p.tokens; t += p.cluster)
-					{
-						float v = 0.0f, u = 0.0f;
-						for (int s = 0; s < p.cluster; s++)
-						{
-							v += ld_shared_cluster_f32(map_to_cta(smem_base + (t * 128 + row) * 4, s));
-							if (KIND == GATED)
-								u += ld_shared_cluster_f32(map_to_cta(smem_base + ((p.tokens + t) * 128 + row) * 4, s));
-						}
+					{ // all loads of a token (from up to eight SMs) before the first addition
+						float v[MAX_CLUSTER], u[KIND == GATED ? MAX_CLUSTER : 1];
+#pragma unroll
+						for (int k = 0; k < MAX_CLUSTER; k++)
+							if (k < p.cluster)
+							{
+								v[k] = ld_shared_cluster_f32(from[k] + t * 512);
+								if (KIND == GATED)
+									u[KIND == GATED ? k : 0] = ld_shared_cluster_f32(from[k] + (p.tokens + t) * 512);
+							}
+#pragma unroll
+						for (int k = 1; k < MAX_CLUSTER; k++)
+							if (k < p.cluster)
+							{
+								v[0] += v[k];
+								if (KIND == GATED)
+									u[0] += u[KIND == GATED ? k : 0];
+							}
 						__half *dst = p.out + static_cast<long long>(t) * p.ldo + n;
 						if (KIND == GATED)
-							*dst = __float2half_rn(gate_value<GATE, true>(v) * u);
+							*dst = __float2half_rn(gate_value<GATE, true>(v[0]) * u[0]);
 						else
-							*dst = __float2half_rn(p.beta != 0.0f ? v + p.beta * __half2float(*dst) : v);
+							*dst = __float2half_rn(p.beta != 0.0f ? v[0] + p.beta * __half2float(*dst) : v[0]);
 					}
+				}
 				cluster_sync(); // no CTA's shared memory goes while another reads it
 			}
 			if (KIND == STATISTICS)
