@@ -310,8 +310,8 @@ void mb200_layernorm_backward(mlContext_t context, const mlTensor_t x, const mlT
 
 /* Gated feed-forward block: y = (act(x Wg^T) * (x Wu^T)) W2^T + beta * y with W1 = [Wg; Wu], a [2 hidden, embed] matrix (gate rows first), and
  * W2 [embed, hidden].  `gate` names act.  `saved` (optional, fp32 [tokens, 2 hidden]) is where the forward pass may leave what its backward
- * pass reads instead of computing it again; its contents are the library's own.  Where making it again is cheaper (fp16 with embed up to
- * 1024 or hidden no multiple of 8) it is left as it was: such a caller need not provide it. */
+ * pass reads instead of computing it again; its contents are the library's own.  (For fp16 with embed up to 1024 making most of it again is
+ * cheaper, and little of it is used: a caller short of memory loses a tenth of the speed without it.) */
 #define MB200_GATE_SIGMOID 0
 #define MB200_GATE_RELU 1
 #define MB200_GATE_SILU 2

@@ -80,6 +80,7 @@ namespace mb200
 				PairResult result; // STORE
 				int direct; // STORE: element-wise stores, for results that TMA cannot address
 				int accumulate; // SUMS
+				int store_h; // GATED_RECOMPUTE
 				float *kept; // a and u: written by GATED unless null, read by GATED_BACKWARD
 				const int *targets;
 				const float *row_weights, *lse;
@@ -586,7 +587,8 @@ namespace mb200
 								const uint32_t at = staging + c * 3 * HALF_BOX + lane * 64 + ((k ^ ((lane >> 1) & 3)) * 16);
 								st_shared_v4(at, pack_half8(da));
 								st_shared_v4(at + HALF_BOX, pack_half8(du));
-								st_shared_v4(at + 2 * HALF_BOX, pack_half8(h));
+								if (p.store_h)
+									st_shared_v4(at + 2 * HALF_BOX, pack_half8(h));
 							}
 						}
 						publish();
@@ -598,7 +600,8 @@ namespace mb200
 								{
 									tma_store_2d(&map_d, staging + c * 3 * HALF_BOX, n + c * 32, row0);
 									tma_store_2d(&map_e, staging + (c * 3 + 1) * HALF_BOX, n + c * 32, row0);
-									tma_store_2d(&map_f, staging + (c * 3 + 2) * HALF_BOX, n + c * 32, row0);
+									if (p.store_h)
+										tma_store_2d(&map_f, staging + (c * 3 + 2) * HALF_BOX, n + c * 32, row0);
 								}
 							bulk_commit_group();
 						}
@@ -1053,9 +1056,10 @@ namespace mb200
 		Params p;
 		if (!prepare(ctx, maps, p, tokens, hidden, embed, x, w1, 2 * hidden, BN / 2, 1) || !map_operand(ctx, &maps.dy, dy, tokens, embed) || !map_operand(ctx, &maps.w2, w2, hidden, embed)
 				|| !map_halves(ctx, &maps.d, dau, 2 * hidden, tokens, hidden) || !map_halves(ctx, &maps.e, dau + hidden, 2 * hidden, tokens, hidden)
-				|| !map_halves(ctx, &maps.f, h, hidden, tokens, hidden))
+				|| (h != nullptr && !map_halves(ctx, &maps.f, h, hidden, tokens, hidden)))
 			return false;
 		p.up_row = hidden;
+		p.store_h = h != nullptr;
 		return with_gate(gate, [&](auto g)
 		{
 			return launch<GATED_RECOMPUTE, decltype(g)::value>(ctx, maps, p);

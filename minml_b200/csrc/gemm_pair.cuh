@@ -45,7 +45,7 @@ namespace mb200
 	 * multiple of 8. */
 	bool pair_gated_backward(mlContext_t ctx, int tokens, int embed, int hidden, const PairOperand &dy, const PairOperand &w2, int gate, const float *kept, __half *dau, __half *h);
 
-	/* The same with nothing kept: a and u are made again, in the same tiles as dh.  dy [tokens, embed] and w2 stored [embed, hidden] (mn). */
+	/* The same with nothing kept: a and u are made again, in the same tiles as dh; h may be null (not wanted).  dy [tokens, embed] and w2 stored [embed, hidden] (mn). */
 	bool pair_gated_recompute(mlContext_t ctx, int tokens, int embed, int hidden, const PairOperand &x, const PairOperand &w1, const PairOperand &dy, const PairOperand &w2, int gate, __half *dau,
 			__half *h);
 
