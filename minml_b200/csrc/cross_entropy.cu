@@ -141,8 +141,8 @@ namespace mb200
 				int c;
 				walk.place(i, t, c);
 				c *= 4;
-				const int target = rows.targets[t] - first - c;
 				const float weight = rows.weight(t), l = lse[t], factor = alpha * weight;
+				const int target = weight != 0.0f ? rows.targets[t] - first - c : -1; // (a row that takes no part may name any number)
 				float4 *at = reinterpret_cast<float4*>(z + t * pitch + c);
 				float4 v = *at;
 				if (weight == 0.0f)

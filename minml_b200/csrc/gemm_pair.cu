@@ -434,7 +434,7 @@ namespace mb200
 						if (!ok)
 							break;
 						const int n0 = u.nt * BN + half * (BN / 2), valid = p.N - n0;
-						const int at = row_ok ? p.targets[row] - n0 : -1;
+						const int wanted = row_ok ? p.targets[row] : -1, at = wanted >= n0 ? wanted - n0 : -1;
 						float top = -INFINITY, sum = 0.0f, target = 0.0f;
 #pragma unroll
 						for (int j = 0; j < BN / 2; j++)
@@ -466,7 +466,7 @@ namespace mb200
 						target = row_ok ? p.targets[row] : -1;
 						active = target >= 0 && target < p.vocab && (p.row_weights == nullptr || p.row_weights[row] != 0.0f);
 						shift = row_ok ? fmaf(p.lse[row], -LOG2E, 15.0f) : 0.0f; // 2^15 exp(z - lse) = 2^(z log2 e + shift)
-						target -= p.first;
+						target = active ? target - p.first : -1;
 					}
 					if (EPI == STORE)
 					{
