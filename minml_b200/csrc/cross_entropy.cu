@@ -23,6 +23,7 @@
 #include "gemm_pair.cuh"
 #include "gemm_fp32.cuh"
 #include "few_tokens.cuh"
+#include "few_rows.cuh"
 
 #include <algorithm>
 
@@ -220,9 +221,20 @@ namespace mb200
 			return static_cast<int>(std::max<long long>(1, std::min<long long>(rows, static_cast<long long>(get(ctx)->sm_count) * 8)));
 		}
 
+		/* Forward: rows are read in place by few_rows.cu; in fp16 only where the weights would be copied. */
+		bool by_few_rows(const Problem &q)
+		{
+			return q.dtype == DTYPE_FLOAT32 ? q.tokens <= FEW_ROWS_FP32 : q.tokens <= FEW_ROWS_FP16 && q.embed % 8 != 0;
+		}
 		int statistics_groups(mlContext_t ctx, const Problem &q)
 		{
+			if (by_few_rows(q))
+				return few_rows_statistics_parts(ctx, static_cast<int>(q.tokens), q.vocab, q.embed);
 			return q.tokens <= FEW_TOKENS ? few_statistics_parts(ctx, q.vocab) : pair_statistics_parts(q.vocab);
+		}
+		bool in_pieces(const Problem &q, bool training)
+		{ // the forward pass in fp16, or of a few rows, keeps 8 bytes for every row and 128 (or 4 to 64) columns and has no use for pieces
+			return training || (q.dtype == DTYPE_FLOAT32 && !by_few_rows(q));
 		}
 		/* The workspace of one call with pieces of `piece` columns. */
 		struct Plan
@@ -230,7 +242,7 @@ namespace mb200
 				int embed; // padded to a pitch that TMA can address
 				int piece, pitch; // columns of a piece of logits or probabilities, and its rows' pitch
 				int dx_splits; // fp32 sums that dx is kept in until the last piece
-				float2 *running = nullptr; // fp32: per row; fp16: per row and 128 columns
+				float2 *running = nullptr; // per row; not in pieces: per row and group of columns
 				float *target_logit = nullptr, *z = nullptr, *dx_sums = nullptr, *partials = nullptr, *largest = nullptr;
 				void *p = nullptr, *x = nullptr, *w = nullptr, *weighted_x = nullptr;
 				size_t bytes = 0;
@@ -243,6 +255,13 @@ namespace mb200
 					piece = columns;
 					pitch = round_up(columns, 64);
 					dx_splits = half && training ? pair_splits(ctx, tokens, q.embed, piece) : 1;
+					if (!training && by_few_rows(q))
+					{
+						target_logit = carve.take<float>(q.tokens);
+						running = carve.take<float2>(q.tokens * statistics_groups(ctx, q));
+						bytes = carve.used;
+						return;
+					}
 					const size_t cells = static_cast<size_t>(q.tokens) * pitch, rows = static_cast<size_t>(q.tokens) * embed;
 					if (embed != q.embed)
 					{
@@ -278,10 +297,6 @@ namespace mb200
 					bytes = carve.used;
 				}
 		};
-		bool in_pieces(const Problem &q, bool training)
-		{ // the forward pass in fp16 keeps 8 bytes for every row and 128 columns and has no use for pieces
-			return training || q.dtype == DTYPE_FLOAT32;
-		}
 		/* Pieces of equal width, multiples of 256 columns, of at most about PIECE_BYTES. */
 		int recommended_piece(const Problem &q, bool training)
 		{
@@ -366,6 +381,20 @@ namespace mb200
 			return false;
 		}
 
+		void join_statistics(mlContext_t ctx, const Problem &q, const Rows &rows, const Plan &plan, float *loss, float *lse)
+		{
+			const cudaError_t status = launch_overlapped(kernel_join_statistics, dim3(static_cast<int>(q.tokens)), dim3(256), 0, use_stream(ctx), plan.running, statistics_groups(ctx, q),
+					plan.target_logit, rows, loss, lse);
+			MB200_COUNT_LAUNCH();
+			check_cuda(ctx, status, "mb200_softmax_cross_entropy_forward");
+		}
+		template<typename T>
+		void forward_few_rows(mlContext_t ctx, const Problem &q, const Rows &rows, const Plan &plan, const mlTensor_t &x, const mlTensor_t &w, float *loss, float *lse)
+		{
+			const FewRows<T> operands { static_cast<int>(q.tokens), q.embed, reinterpret_cast<const T*>(x.data), reinterpret_cast<const T*>(w.data) };
+			if (few_rows_statistics(ctx, operands, q.vocab, rows.targets, plan.running, plan.target_logit))
+				join_statistics(ctx, q, rows, plan, loss, lse);
+		}
 		void forward_half(mlContext_t ctx, const Problem &q, const Rows &rows, const Plan &plan, const Operands<__half> &o, float *loss, float *lse)
 		{
 			const int tokens = static_cast<int>(q.tokens);
@@ -373,12 +402,8 @@ namespace mb200
 					? few_statistics(ctx, FewTokens { tokens, plan.embed, o.x, plan.embed, o.w, plan.embed }, q.vocab, rows.targets, plan.running, plan.target_logit)
 					: pair_statistics(ctx, tokens, q.vocab, q.embed, PairOperand { o.x, plan.embed, false }, PairOperand { o.w, plan.embed, false }, rows.targets, plan.running,
 							plan.target_logit);
-			if (!ok)
-				return;
-			const cudaError_t status = launch_overlapped(kernel_join_statistics, dim3(tokens), dim3(256), 0, use_stream(ctx), plan.running, statistics_groups(ctx, q), plan.target_logit, rows,
-					loss, lse);
-			MB200_COUNT_LAUNCH();
-			check_cuda(ctx, status, "mb200_softmax_cross_entropy_forward");
+			if (ok)
+				join_statistics(ctx, q, rows, plan, loss, lse);
 		}
 		void forward_float(mlContext_t ctx, const Problem &q, const Rows &rows, const Plan &plan, const Operands<float> &o, float *loss, float *lse)
 		{
@@ -500,12 +525,16 @@ extern "C"
 		if (piece == 0)
 			return;
 		const Plan plan(context, q, workspace.data, false, piece);
-		if (!check_alignment(context, who, "x", x, plan.x != nullptr) || !check_alignment(context, who, "weights", w, plan.x != nullptr))
+		if (!check_alignment(context, who, "x", x, plan.embed != q.embed) || !check_alignment(context, who, "weights", w, plan.embed != q.embed))
 			return;
 		flush_pending(context);
 		const Rows rows { reinterpret_cast<const int*>(targets.data), nullptr, q.vocab };
 		float *loss_data = reinterpret_cast<float*>(loss.data), *lse_data = reinterpret_cast<float*>(lse.data);
-		if (q.dtype == DTYPE_FLOAT16)
+		if (by_few_rows(q) && q.dtype == DTYPE_FLOAT16)
+			forward_few_rows<__half>(context, q, rows, plan, x, w, loss_data, lse_data);
+		else if (by_few_rows(q))
+			forward_few_rows<float>(context, q, rows, plan, x, w, loss_data, lse_data);
+		else if (q.dtype == DTYPE_FLOAT16)
 			forward_half(context, q, rows, plan, Operands<__half>(context, q, plan, x, w), loss_data, lse_data);
 		else
 			forward_float(context, q, rows, plan, Operands<float>(context, q, plan, x, w), loss_data, lse_data);

@@ -17,6 +17,7 @@
 #include "gemm_pair.cuh"
 #include "gemm_fp32.cuh"
 #include "few_tokens.cuh"
+#include "few_rows.cuh"
 
 #include <algorithm>
 
@@ -117,6 +118,7 @@ namespace mb200
 		{
 				int embed, hidden; // padded
 				bool pack_x, pack_w1, pack_w2;
+				bool few_rows; // the forward pass goes by few_rows.cu, which reads all rows in place
 				bool keeps, keeps_h; // what the forward pass leaves in `saved`: a and u, or h, or nothing
 				void *x = nullptr, *w1 = nullptr, *w2 = nullptr, *dy = nullptr, *h = nullptr, *dau = nullptr;
 				float *au = nullptr, *dh = nullptr, *partials = nullptr;
@@ -132,8 +134,16 @@ namespace mb200
 					pack_w1 = pack_x || hidden != p.hidden;
 					pack_w2 = hidden != p.hidden;
 					keeps = saved && (p.dtype == DTYPE_FLOAT32 || (hidden == p.hidden && p.embed > RECOMPUTE_UP_TO));
+					// in fp16 only where weights would be copied, and not where `saved` has the form that the tensor-core tile of the backward pass reads
+					few_rows = !backward && (p.dtype == DTYPE_FLOAT32 ? p.tokens <= FEW_ROWS_FP32 : p.tokens <= FEW_ROWS_FP16 && pack_w1 && !saved);
 					keeps_h = saved && !keeps && hidden <= 4 * p.hidden; // a quarter of the room of a and u, unless it is nearly all padding
 					const size_t th = static_cast<size_t>(p.tokens) * hidden, te = static_cast<size_t>(p.tokens) * embed;
+					if (few_rows)
+					{
+						h = carve.take<uint8_t>(th * es);
+						bytes = carve.used;
+						return;
+					}
 					if (pack_x)
 						x = carve.take<uint8_t>(te * es);
 					if (pack_w1)
@@ -289,6 +299,20 @@ namespace mb200
 						product(p.embed, p.hidden, tokens, dy, plan.embed, true, h, F, true, dw2, p.hidden, beta_dw);
 				}
 		};
+		template<typename T>
+		T* data_of(const mlTensor_t &t)
+		{
+			return reinterpret_cast<T*>(t.data);
+		}
+		/* The forward pass where plan.few_rows */
+		template<typename T>
+		void forward_few_rows(mlContext_t ctx, const Problem &p, const Plan &plan, const mlTensor_t &x, const mlTensor_t &w1, const mlTensor_t &w2, T *y, float beta, float *au)
+		{
+			T *h = reinterpret_cast<T*>(plan.h);
+			const int tokens = static_cast<int>(p.tokens);
+			if (few_rows_gated(ctx, FewRows<T> { tokens, p.embed, data_of<T>(x), data_of<T>(w1) }, p.hidden, p.gate, h, au))
+				few_rows_product(ctx, FewRows<T> { tokens, p.hidden, h, data_of<T>(w2) }, p.embed, y, beta);
+		}
 		/* TMA reads operands whose rows need no padding from where they lie. */
 		bool check_alignment(mlContext_t ctx, const char *who, const char *name, const mlTensor_t &t, bool copied)
 		{
@@ -296,11 +320,6 @@ namespace mb200
 				return true;
 			record_error(ctx, "%s: %s must be 16-byte aligned", who, name);
 			return false;
-		}
-		template<typename T>
-		T* data_of(const mlTensor_t &t)
-		{
-			return reinterpret_cast<T*>(t.data);
 		}
 
 		bool check_problem(mlContext_t ctx, const char *who, const mlTensor_t &x, const mlTensor_t &w1, const mlTensor_t &w2, int gate, Problem &p)
@@ -380,7 +399,11 @@ extern "C"
 					return;
 		}
 		flush_pending(context);
-		if (p.dtype == DTYPE_FLOAT16)
+		if (plan.few_rows && p.dtype == DTYPE_FLOAT16)
+			forward_few_rows<__half>(context, p, plan, x, w1, w2, data_of<__half>(y), beta, nullptr);
+		else if (plan.few_rows)
+			forward_few_rows<float>(context, p, plan, x, w1, w2, data_of<float>(y), beta, data_of<float>(saved));
+		else if (p.dtype == DTYPE_FLOAT16)
 			Run<__half>(context, p, plan, x, w1, w2, no_tensor()).forward(data_of<__half>(y), beta, data_of<float>(saved));
 		else
 			Run<float>(context, p, plan, x, w1, w2, no_tensor()).forward(data_of<float>(y), beta, data_of<float>(saved));

@@ -143,6 +143,40 @@ def test_rows_left_out_may_hold_anything(ctx, dtype, tokens):
     want_dw.holds(dw, dtype)
 
 
+@pytest.mark.parametrize("tokens", [1, 2, 3, 4, 5, 8, 9, 16])
+@pytest.mark.parametrize("embed,vocab", [(516, 3001), (1030, 77), (2049, 5), (33, 9000)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_few_tokens_of_any_row_length(ctx, dtype, embed, vocab, tokens):
+    from minml_b200 import backend as B
+    x, w, targets, _ = make(tokens + vocab, tokens, embed, vocab, dtype)
+    targets[-1] = vocab - 1
+    want_loss, want_lse, *_ = forward(x, w, targets)
+    around = torch.full((2, tokens + 2), 7.0, device="cuda")
+    loss, lse = around[0, 1:-1], around[1, 1:-1]
+    size = B.softmaxCrossEntropyGetWorkspaceSize(ctx, x.shape, w.shape, dtype, False)
+    B.softmaxCrossEntropyForward(ctx, x, w, targets, loss, lse, torch.full((size,), 255, device="cuda", dtype=torch.uint8))
+    ctx.synchronize()
+    want_loss.holds(loss)
+    want_lse.holds(lse)
+    assert bool((around[:, 0] == 7.0).all()) and bool((around[:, -1] == 7.0).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("tokens,embed,vocab", [(3, 64, 700), (3, 66, 700), (40, 64, 700), (140, 64, 700)])
+def test_targets_at_the_ends_of_their_type(ctx, dtype, tokens, embed, vocab):
+    """The least and the largest int32 are outside the vocabulary like any other such value: no arithmetic on them may come round to a column."""
+    x, w, targets, _ = make(5, tokens, embed, vocab, dtype, 0.0)
+    targets[0], targets[-1] = -2 ** 31, 2 ** 31 - 1
+    want_loss, want_lse, *_ = forward(x, w, targets)
+    want_dx, want_dw = backward(x, w, targets, 16.0)
+    loss, lse, dx, dw = run(ctx, x, w, targets, 16.0)
+    want_loss.holds(loss)
+    want_lse.holds(lse)
+    want_dx.holds(dx, dtype)
+    want_dw.holds(dw, dtype)
+    assert float(loss[0]) == 0.0 and float(loss[-1]) == 0.0 and not bool(dx[0].any()) and not bool(dx[-1].any())
+
+
 def test_no_row_takes_part(ctx):
     x, w, targets, _ = make(9, 130, 64, 300, torch.float16, 2.0)
     assert int(targets.max()) == -1

@@ -126,6 +126,44 @@ def test_backward(ctx, dtype, tokens, embed, hidden):
     (want_dw2 + Bounded(old_2).scaled(0.5)).holds(dw2, dtype)
 
 
+@pytest.mark.parametrize("tokens", [1, 2, 3, 4, 5, 8, 9, 16])
+@pytest.mark.parametrize("embed,hidden", [(516, 1028), (1030, 514), (2049, 131), (33, 2051)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_few_tokens_of_any_row_length(ctx, dtype, embed, hidden, tokens):
+    """Rows read by fours, by twos and singly, short and shared by several warps; the memory around y is left as it was."""
+    from minml_b200 import backend as B
+    x, w1, w2, old = make(tokens + embed, tokens, embed, hidden, dtype)
+    around = torch.full((tokens + 2, embed), 7.0, device="cuda", dtype=dtype)
+    y = around.view(-1)[embed:-embed].view(tokens, embed)
+    if y.data_ptr() % 16:  # (results need their element's alignment only)
+        assert embed % 8
+    for kind, beta in (("silu", 0.0), ("gelu", -1.5)):
+        _, want, *_ = forward(x, w1, w2, kind)
+        y.copy_(old)
+        B.gatedFeedForwardForward(ctx, x, w1, w2, y, kind, beta=beta, workspace=workspace(ctx, x, w1, False))
+        ctx.synchronize()
+        (want if beta == 0.0 else want + Bounded(old).scaled(beta)).holds(y, dtype)
+        assert bool((around[0] == 7.0).all()) and bool((around[-1] == 7.0).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_few_tokens_off_their_alignment(ctx, dtype):
+    """Padded operands may begin at any element, also where their row length alone would allow wider reads."""
+    from minml_b200 import backend as B
+    tokens, embed, hidden = 3, 52 if dtype == torch.float16 else 50, 66
+    x, w1, w2, _ = make(11, tokens, embed, hidden, dtype)
+    _, want, *_ = forward(x, w1, w2, "silu")
+    shifted = []
+    for t in (x, w1, w2):
+        buffer = torch.zeros(t.numel() + 1, device="cuda", dtype=dtype)
+        buffer[1:] = t.view(-1)
+        shifted.append(buffer[1:].view(t.shape))
+    y = nan_like(x)
+    B.gatedFeedForwardForward(ctx, *shifted, y, "silu", workspace=workspace(ctx, x, w1, False))
+    ctx.synchronize()
+    want.holds(y, dtype)
+
+
 def test_the_formulas_against_differences():
     """act' and the backward formulas in fp64, against central differences of the forward formula."""
     torch.manual_seed(1)
