@@ -30,13 +30,20 @@ namespace mb200
 		using namespace epi;
 
 		constexpr int BM = 128, BN = 128, BK = 32;
-		constexpr int OPERAND_BYTES = 128 * 128;
-		constexpr int STAGE_BYTES = 2 * OPERAND_BYTES;
-		constexpr int STAGES = 4, LO_STAGES = 2, BUFFERS = 4;
-		constexpr int EPI_WARPS = 8, SPLIT_WARPS = 4;
-		constexpr int THREADS = (2 + EPI_WARPS + SPLIT_WARPS) * 32;
+		constexpr int A_BYTES = BM * BK * 4, B_BYTES = BN / 2 * BK * 4; // of a CTA
+		constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+		constexpr int STAGES = 6, LO_STAGES = 4, BUFFERS = 2;
+		constexpr int A_COLUMNS = 2 * BK; // of tensor memory: hi and lo of a stage of A, a row a lane
+		constexpr int TMEM_COLUMNS = 512;
+		static_assert(BUFFERS * BN + LO_STAGES * A_COLUMNS <= TMEM_COLUMNS, "tensor memory");
+		constexpr int EPI_FIRST = 4, EPI_WARPS = 8, SPLIT_FIRST = EPI_FIRST + EPI_WARPS, SPLIT_WARPS = 4, SPLIT_GROUPS = 2; // groups take stages in turn
+		constexpr int THREADS = (SPLIT_FIRST + SPLIT_WARPS * SPLIT_GROUPS) * 32;
+		// warps 0-3, the epilogue's and the split's; launched with 96 registers a thread
+		constexpr int REGISTERS_FEW = 40, REGISTERS_EPILOGUE = 144, REGISTERS_SPLIT = 72;
+		static_assert(128 * REGISTERS_FEW + 256 * REGISTERS_EPILOGUE + 256 * REGISTERS_SPLIT <= THREADS * 96, "registers of the block at launch");
+		constexpr int BOX_MN_BYTES = BK * 128; // 32 rows of an operand that is stored [K, rows]
 		constexpr int BOX_BYTES = 32 * 128; // per epilogue warp: 32 x 32 results
-		constexpr int SMEM_BYTES = (STAGES + LO_STAGES) * STAGE_BYTES + EPI_WARPS * BOX_BYTES + 1024;
+		constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + LO_STAGES * B_BYTES + EPI_WARPS * BOX_BYTES + 1024;
 
 		struct Params
 		{
@@ -70,7 +77,9 @@ namespace mb200
 			const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
 			const uint32_t lo_base = smem_base + STAGES * STAGE_BYTES;
 			const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-			const int tiles = p.m_tiles * p.n_tiles, units = tiles * p.splits;
+			const uint32_t rank = cluster_ctarank();
+			const bool leader = rank == 0;
+			const int tiles = p.m_tiles * p.n_tiles, units = tiles * p.splits, first_unit = blockIdx.x / 2, unit_step = gridDim.x / 2;
 			struct Unit
 			{
 					int m0, n0, kb0, kb1, split;
@@ -80,7 +89,7 @@ namespace mb200
 				Unit u;
 				u.split = unit / tiles;
 				const int rest = unit - u.split * tiles;
-				u.m0 = rest / p.n_tiles * BM;
+				u.m0 = (rest / p.n_tiles * 2 + static_cast<int>(rank)) * BM;
 				u.n0 = rest % p.n_tiles * BN;
 				u.kb0 = u.split * p.blocks_per_split;
 				u.kb1 = min(p.k_blocks, u.kb0 + p.blocks_per_split);
@@ -92,7 +101,7 @@ namespace mb200
 				for (int s = 0; s < STAGES; s++)
 				{
 					mbar_init(smem_u32(&bars.full[s]), 1);
-					mbar_init(smem_u32(&bars.split[s]), SPLIT_WARPS);
+					mbar_init(smem_u32(&bars.split[s]), 2 * SPLIT_WARPS);
 					mbar_init(smem_u32(&bars.empty[s]), 1);
 				}
 				for (int s = 0; s < LO_STAGES; s++)
@@ -100,18 +109,18 @@ namespace mb200
 				for (int b = 0; b < BUFFERS; b++)
 				{
 					mbar_init(smem_u32(&bars.tmem_full[b]), 1);
-					mbar_init(smem_u32(&bars.tmem_empty[b]), EPI_WARPS);
+					mbar_init(smem_u32(&bars.tmem_empty[b]), 2 * EPI_WARPS);
 				}
 				bars.abort_flag = 0;
 				fence_mbar_init();
 			}
 			if (warp == 1)
 			{
-				tmem_alloc(smem_u32(&bars.tmem_base), BUFFERS * BN);
-				tmem_relinquish();
+				asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(&bars.tmem_base)), "r"(TMEM_COLUMNS) : "memory");
+				asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
 			}
 			tcgen05_fence_before();
-			__syncthreads();
+			cluster_sync(); // the peer's barriers exist before anything signals them
 			tcgen05_fence_after();
 			const uint32_t tmem_base = bars.tmem_base;
 			volatile int *abort_flag = &bars.abort_flag;
@@ -120,13 +129,14 @@ namespace mb200
 
 			if (warp == 0)
 			{ /* ------------------------------------------------ operands */
+				asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(REGISTERS_FEW));
 				if (elect_one())
 				{
 					prefetch_tensormap(&map_a);
 					prefetch_tensormap(&map_b);
 					uint32_t it = 0;
 					bool ok = true;
-					for (int unit = blockIdx.x; unit < units && ok; unit += gridDim.x)
+					for (int unit = first_unit; unit < units && ok; unit += unit_step)
 					{
 						const Unit u = locate(unit);
 						for (int kb = u.kb0; kb < u.kb1; kb++, it++)
@@ -139,23 +149,24 @@ namespace mb200
 							}
 							const uint32_t full = smem_u32(&bars.full[s]);
 							mbar_arrive_expect_tx(full, STAGE_BYTES);
-							const uint32_t a = smem_base + s * STAGE_BYTES, b = a + OPERAND_BYTES;
+							const uint32_t a = smem_base + s * STAGE_BYTES, b = a + A_BYTES;
+							const int n0 = u.n0 + static_cast<int>(rank) * (BN / 2); // this CTA's half of the columns
 							if (p.a_mn)
 							{
 #pragma unroll
 								for (int j = 0; j < 4; j++)
-									tma_load_3d(a + j * (OPERAND_BYTES / 4), &map_a, full, u.m0 + j * 32, kb * BK, 0);
+									tma_load_3d(a + j * BOX_MN_BYTES, &map_a, full, u.m0 + j * 32, kb * BK, 0);
 							}
 							else
 								tma_load_3d(a, &map_a, full, kb * BK, u.m0, 0);
 							if (p.b_mn)
 							{
 #pragma unroll
-								for (int j = 0; j < 4; j++)
-									tma_load_3d(b + j * (OPERAND_BYTES / 4), &map_b, full, u.n0 + j * 32, kb * BK, 0);
+								for (int j = 0; j < 2; j++)
+									tma_load_3d(b + j * BOX_MN_BYTES, &map_b, full, n0 + j * 32, kb * BK, 0);
 							}
 							else
-								tma_load_3d(b, &map_b, full, kb * BK, u.n0, 0);
+								tma_load_3d(b, &map_b, full, kb * BK, n0, 0);
 						}
 					}
 				}
@@ -163,24 +174,26 @@ namespace mb200
 			}
 			else if (warp == 1)
 			{ /* ------------------------------------------- multiplications */
-				if (elect_one())
+				asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(REGISTERS_FEW));
+				if (leader && elect_one())
 				{
-					const uint32_t idesc = make_idesc_tf32(BN) | (p.a_mn ? (1u << 15) : 0u) | (p.b_mn ? (1u << 16) : 0u);
-					// per instruction (8 K indices), in 16-byte units: 32 bytes along K, or 8 K indices of 128 bytes
-					const uint32_t step_a = p.a_mn ? 64 : 2, step_b = p.b_mn ? 64 : 2;
-					auto describe = [](uint32_t addr, bool mn) -> uint64_t
+					const uint32_t idesc = make_idesc_tf32_pair(BN) | (p.b_mn ? (1u << 16) : 0u);
+					// per instruction (8 K indices): 8 columns of A; of B, in 16-byte units, 32 bytes along K, or 8 K indices of 128 bytes
+					const uint32_t step_b = p.b_mn ? 64 : 2;
+					auto describe = [&](uint32_t addr) -> uint64_t
 					{
-						return mn ? make_desc_mn_sw128(addr, OPERAND_BYTES / 4, true) : make_desc_k_sw128(addr);
+						return p.b_mn ? make_desc_mn_sw128(addr, BOX_MN_BYTES, true) : make_desc_k_sw128(addr);
 					};
 					uint32_t it = 0;
 					bool ok = true;
-					for (int unit = blockIdx.x; unit < units && ok; unit += gridDim.x)
+					for (int unit = first_unit; unit < units && ok; unit += unit_step)
 					{
 						const Unit u = locate(unit);
 						for (int kb = u.kb0; kb < u.kb1; kb++, it++)
 						{
 							const int s = it % STAGES, b = it % BUFFERS;
-							if (!mbar_wait(smem_u32(&bars.tmem_empty[b]), ((it / BUFFERS) & 1u) ^ 1u, abort_flag) || !mbar_wait(smem_u32(&bars.split[s]), (it / STAGES) & 1u, abort_flag))
+							if (!mbar_wait_cluster(smem_u32(&bars.tmem_empty[b]), ((it / BUFFERS) & 1u) ^ 1u, abort_flag)
+									|| !mbar_wait_cluster(smem_u32(&bars.split[s]), (it / STAGES) & 1u, abort_flag))
 							{
 								ok = false;
 								break;
@@ -188,69 +201,108 @@ namespace mb200
 							tcgen05_fence_after();
 							fence_proxy_async_smem(); // lo was written by plain stores of the split warps
 							const uint32_t d = tmem_base + b * BN;
-							const uint32_t hi = smem_base + s * STAGE_BYTES, lo = lo_base + (it % LO_STAGES) * STAGE_BYTES;
-							const uint64_t hi_a = describe(hi, p.a_mn), hi_b = describe(hi + OPERAND_BYTES, p.b_mn);
-							const uint64_t lo_a = describe(lo, p.a_mn), lo_b = describe(lo + OPERAND_BYTES, p.b_mn);
+							const uint32_t hi_a = tmem_base + BUFFERS * BN + (it % LO_STAGES) * A_COLUMNS, lo_a = hi_a + BK;
+							const uint64_t hi_b = describe(smem_base + s * STAGE_BYTES + A_BYTES), lo_b = describe(lo_base + (it % LO_STAGES) * B_BYTES);
 							// the small products first: their sum is cut at its own size
 #pragma unroll
 							for (int k = 0; k < 4; k++)
-								mma_ss<2>(d, hi_a + step_a * k, lo_b + step_b * k, idesc, k > 0 ? 1u : 0u);
+								mma_ts_tf32_pair(d, hi_a + 8 * k, lo_b + step_b * k, idesc, k > 0 ? 1u : 0u);
 #pragma unroll
 							for (int k = 0; k < 4; k++)
-								mma_ss<2>(d, lo_a + step_a * k, hi_b + step_b * k, idesc, 1u);
-							mma_commit(smem_u32(&bars.lo_empty[it % LO_STAGES]));
+								mma_ts_tf32_pair(d, lo_a + 8 * k, hi_b + step_b * k, idesc, 1u);
 #pragma unroll
 							for (int k = 0; k < 4; k++)
-								mma_ss<2>(d, hi_a + step_a * k, hi_b + step_b * k, idesc, 1u);
-							mma_commit(smem_u32(&bars.empty[s]));
-							mma_commit(smem_u32(&bars.tmem_full[b]));
+								mma_ts_tf32_pair(d, hi_a + 8 * k, hi_b + step_b * k, idesc, 1u);
+							mma_commit_pair(smem_u32(&bars.lo_empty[it % LO_STAGES]));
+							mma_commit_pair(smem_u32(&bars.empty[s]));
+							mma_commit_pair(smem_u32(&bars.tmem_full[b]));
 						}
 					}
 				}
 				__syncwarp();
 			}
-			else if (warp >= 2 + EPI_WARPS)
-			{ /* ------------------------------------------- split: lo of every element */
-				const int t = threadIdx.x - (2 + EPI_WARPS) * 32;
+			else if (warp < EPI_FIRST)
+				asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(REGISTERS_FEW));
+			else if (warp >= SPLIT_FIRST)
+			{ /* ------------------------------------------- split: A to tensor memory, lo of B to shared memory */
+				asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(REGISTERS_SPLIT));
+				const int t = threadIdx.x % (SPLIT_WARPS * 32), q = warp % 4;
+				const uint32_t group = (warp - SPLIT_FIRST) / SPLIT_WARPS;
 				uint32_t it = 0;
 				bool ok = true;
-				for (int unit = blockIdx.x; unit < units && ok; unit += gridDim.x)
+				for (int unit = first_unit; unit < units && ok; unit += unit_step)
 				{
 					const Unit u = locate(unit);
 					for (int kb = u.kb0; kb < u.kb1; kb++, it++)
 					{
 						const int s = it % STAGES;
-						if (!mbar_wait(smem_u32(&bars.lo_empty[it % LO_STAGES]), ((it / LO_STAGES) & 1u) ^ 1u, abort_flag) || !mbar_wait(smem_u32(&bars.full[s]), (it / STAGES) & 1u, abort_flag))
+						if (it % SPLIT_GROUPS != group)
+							continue;
+						if (!mbar_wait_all_lanes(smem_u32(&bars.lo_empty[it % LO_STAGES]), ((it / LO_STAGES) & 1u) ^ 1u, abort_flag)
+								|| !mbar_wait_all_lanes(smem_u32(&bars.full[s]), (it / STAGES) & 1u, abort_flag))
 						{
 							ok = false;
 							break;
 						}
-						const uint32_t hi = smem_base + s * STAGE_BYTES, lo = lo_base + (it % LO_STAGES) * STAGE_BYTES;
-						constexpr int PER_THREAD = STAGE_BYTES / 16 / (SPLIT_WARPS * 32), GROUP = 8;
-#pragma unroll 1
-						for (int g = 0; g < PER_THREAD; g += GROUP)
-						{ // elementwise, so whatever swizzle the copy wrote is kept
-							uint4 x[GROUP];
+						tcgen05_fence_after();
+						const uint32_t a = smem_base + s * STAGE_BYTES, hi = a + A_BYTES, lo = lo_base + (it % LO_STAGES) * B_BYTES;
+						const uint32_t to = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + BUFFERS * BN + (it % LO_STAGES) * A_COLUMNS;
+						// a lane's row of A, 16 K indices at a time
 #pragma unroll
-							for (int i = 0; i < GROUP; i++)
-								x[i] = ld_shared_v4(hi + (t + (g + i) * SPLIT_WARPS * 32) * 16);
+						for (int c = 0; c < BK; c += 16)
+						{
+							uint32_t x[16], low[16];
+							if (p.a_mn)
+							{ // [block of 32 rows][K index][row]
 #pragma unroll
-							for (int i = 0; i < GROUP; i++)
-								st_shared_v4(lo + (t + (g + i) * SPLIT_WARPS * 32) * 16, make_uint4(low_part(x[i].x), low_part(x[i].y), low_part(x[i].z), low_part(x[i].w)));
+								for (int k = 0; k < 16; k++)
+									x[k] = __float_as_uint(ld_shared_f32(a + q * BOX_MN_BYTES + (c + k) * 128 + lane * 4));
+							}
+							else
+							{ // [row][K index], 16-byte pieces swizzled
+#pragma unroll
+								for (int k = 0; k < 4; k++)
+								{
+									const uint4 v = ld_shared_v4(a + (q * 32 + lane) * 128 + (((c / 4 + k) ^ (lane & 7)) * 16));
+									x[4 * k] = v.x;
+									x[4 * k + 1] = v.y;
+									x[4 * k + 2] = v.z;
+									x[4 * k + 3] = v.w;
+								}
+							}
+#pragma unroll
+							for (int k = 0; k < 16; k++)
+							{
+								low[k] = low_part(x[k]);
+								x[k] &= 0xFFFFE000u;
+							}
+							tmem_st_32x16(to + c, x);
+							tmem_st_32x16(to + BK + c, low);
 						}
+						constexpr int PER_THREAD = B_BYTES / 16 / (SPLIT_WARPS * 32);
+						uint4 x[PER_THREAD]; // of B, elementwise, so whatever swizzle the copy wrote is kept
+#pragma unroll
+						for (int i = 0; i < PER_THREAD; i++)
+							x[i] = ld_shared_v4(hi + (t + i * SPLIT_WARPS * 32) * 16);
+#pragma unroll
+						for (int i = 0; i < PER_THREAD; i++)
+							st_shared_v4(lo + (t + i * SPLIT_WARPS * 32) * 16, make_uint4(low_part(x[i].x), low_part(x[i].y), low_part(x[i].z), low_part(x[i].w)));
+						tmem_wait_st();
+						tcgen05_fence_before();
 						fence_proxy_async_smem();
 						__syncwarp();
 						if (lane == 0)
-							mbar_arrive(smem_u32(&bars.split[s]));
+							arrive_at_leader(smem_u32(&bars.split[s]));
 					}
 				}
 			}
 			else
 			{ /* ------------------------------------------------------------ sums and results */
-				const int q = warp % 4, half = (warp - 2) / 4;
+				asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(REGISTERS_EPILOGUE));
+				const int q = warp % 4, half = (warp - EPI_FIRST) / 4;
 				uint32_t it = 0;
 				bool ok = true;
-				for (int unit = blockIdx.x; unit < units && ok; unit += gridDim.x)
+				for (int unit = first_unit; unit < units && ok; unit += unit_step)
 				{
 					const Unit u = locate(unit);
 					float v[BN / 2];
@@ -260,7 +312,7 @@ namespace mb200
 					for (int kb = u.kb0; kb < u.kb1; kb++, it++)
 					{
 						const int b = it % BUFFERS;
-						if (!mbar_wait_warp(smem_u32(&bars.tmem_full[b]), (it / BUFFERS) & 1u, abort_flag, 20u))
+						if (!mbar_wait_all_lanes(smem_u32(&bars.tmem_full[b]), (it / BUFFERS) & 1u, abort_flag))
 						{
 							ok = false;
 							break;
@@ -274,7 +326,7 @@ namespace mb200
 						tcgen05_fence_before();
 						__syncwarp();
 						if (lane == 0)
-							mbar_arrive(smem_u32(&bars.tmem_empty[b]));
+							arrive_at_leader(smem_u32(&bars.tmem_empty[b]));
 #pragma unroll
 						for (int j = 0; j < 32; j++)
 						{
@@ -286,7 +338,7 @@ namespace mb200
 						break;
 					// a lane holds 64 columns of one row; through shared memory, so that a store instruction covers 128 bytes of one row
 					const int row0 = u.m0 + q * 32, rows = min(32, p.M - row0);
-					const uint32_t box = lo_base + LO_STAGES * STAGE_BYTES + (warp - 2) * BOX_BYTES;
+					const uint32_t box = lo_base + LO_STAGES * B_BYTES + (warp - EPI_FIRST) * BOX_BYTES;
 #pragma unroll
 					for (int c = 0; c < 2; c++)
 					{
@@ -319,10 +371,11 @@ namespace mb200
 					atomicExch(p.status, 1);
 				__nanosleep(1000000); // give copies that are still in flight time to land before the CTA retires
 			}
+			cluster_sync(); // neither CTA's shared or tensor memory goes while the other may still use it
 			if (warp == 1)
 			{
 				tcgen05_fence_after();
-				tmem_dealloc(tmem_base, BUFFERS * BN);
+				asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" :: "r"(tmem_base), "r"(TMEM_COLUMNS) : "memory");
 			}
 		}
 
@@ -372,10 +425,43 @@ namespace mb200
 	/* As pair_splits (gemm_pair.cu), with this kernel's figures: a K block of a tile 0.75 us. */
 	namespace
 	{
+		/* How many clusters the device holds at once; 0 when they cannot be placed.  Also opts the kernel in to its shared memory; both once per device. */
+		int resident_clusters(mlContext_t ctx)
+		{
+			static int known[MAX_DEVICES] = { 0 }; // 0: not asked yet, -1: none
+			static std::mutex mutex;
+			std::lock_guard<std::mutex> lock(mutex);
+			const int device = get(ctx)->device;
+			if (device < 0 || device >= MAX_DEVICES)
+				return 0;
+			if (known[device] == 0)
+			{
+				use_stream(ctx);
+				int n = 0;
+				cudaLaunchConfig_t config = { };
+				cudaLaunchAttribute attribute = { };
+				attribute.id = cudaLaunchAttributeClusterDimension;
+				attribute.val.clusterDim.x = 2;
+				attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+				config.gridDim = dim3(2 * (get(ctx)->sm_count / 2));
+				config.blockDim = dim3(THREADS);
+				config.dynamicSmemBytes = SMEM_BYTES;
+				config.attrs = &attribute;
+				config.numAttrs = 1;
+				if (cudaFuncSetAttribute(kernel_gemm_fp32, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess
+						|| cudaOccupancyMaxActiveClusters(&n, kernel_gemm_fp32, &config) != cudaSuccess || n <= 0)
+				{
+					cudaGetLastError();
+					n = -1;
+				}
+				known[device] = n;
+			}
+			return std::max(0, known[device]);
+		}
 		int float_splits(mlContext_t ctx, int M, int N, int K)
 		{
-			const int sms = get(ctx)->sm_count;
-			const long long tiles = static_cast<long long>((M + BM - 1) / BM) * ((N + BN - 1) / BN);
+			const int clusters = std::max(1, resident_clusters(ctx));
+			const long long tiles = static_cast<long long>((M + 2 * BM - 1) / (2 * BM)) * ((N + BN - 1) / BN);
 			const int k_blocks = (K + BK - 1) / BK;
 			int best = 1;
 			double best_time = 0.0;
@@ -387,7 +473,7 @@ namespace mb200
 				const double partial_bytes = s == 1 ? 0.0 : 8.0 * s * M * N;
 				if (partial_bytes > 2.0 * (size_t(256) << 20))
 					break;
-				const double time = static_cast<double>((tiles * s + sms - 1) / sms) * (blocks * 0.75 + 1.5) + (s == 1 ? 0.0 : 4.0 + partial_bytes / 5.0e6);
+				const double time = static_cast<double>((tiles * s + clusters - 1) / clusters) * (blocks * 0.5 + 1.5) + (s == 1 ? 0.0 : 4.0 + partial_bytes / 5.0e6);
 				if (s == 1 || time < best_time)
 				{
 					best = s;
@@ -408,30 +494,24 @@ namespace mb200
 	}
 	bool float_product(mlContext_t ctx, int M, int N, int K, const FloatOperand &a, const FloatOperand &b, float *d, int ldd, float beta, float *partials)
 	{
-		static bool configured_on[MAX_DEVICES] = { false }; // the opt-in is a per-device attribute of the kernel
-		static std::mutex mutex;
 		Context *c = get(ctx);
-		cudaStream_t stream = use_stream(ctx);
-		if (c->device < 0 || c->device >= MAX_DEVICES)
-			return false;
+		const int resident = resident_clusters(ctx);
+		if (resident == 0)
 		{
-			std::lock_guard<std::mutex> lock(mutex);
-			if (!configured_on[c->device])
-				configured_on[c->device] = check_cuda(ctx, cudaFuncSetAttribute(kernel_gemm_fp32, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES), "gemm_fp32: shared memory opt-in");
-			if (!configured_on[c->device])
-				return false;
+			record_error(ctx, "gemm_fp32: a cluster of two CTAs with %d bytes of shared memory each cannot be placed on this device", SMEM_BYTES);
+			return false;
 		}
 		// an operand stored [rows, K]: boxes of 128 rows x 128 bytes of K; stored [K, rows]: 32 K indices x 128 bytes of rows, whose swizzle moves
 		// 32-byte pieces (tc.cuh)
-		auto encode = [&](CUtensorMap *map, const FloatOperand &o, int rows) -> bool
+		auto encode = [&](CUtensorMap *map, const FloatOperand &o, int rows, uint32_t box_rows, CUtensorMapSwizzle swizzle_mn) -> bool
 		{
 			const uint64_t dims[3] = { static_cast<uint64_t>(o.mn ? rows : K), static_cast<uint64_t>(o.mn ? K : rows), 1 };
 			const uint64_t strides[2] = { static_cast<uint64_t>(o.ld) * 4, static_cast<uint64_t>(o.ld) * 4 * dims[1] };
-			const uint32_t box[3] = { 32, o.mn ? 32u : 128u, 1 };
-			return encode_tensor_map(ctx, map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, o.data, dims, strides, box, o.mn ? CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B : CU_TENSOR_MAP_SWIZZLE_128B);
+			const uint32_t box[3] = { 32, o.mn ? 32u : box_rows, 1 };
+			return encode_tensor_map(ctx, map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, o.data, dims, strides, box, o.mn ? swizzle_mn : CU_TENSOR_MAP_SWIZZLE_128B);
 		};
 		CUtensorMap map_a, map_b;
-		if (!encode(&map_a, a, M) || !encode(&map_b, b, N))
+		if (!encode(&map_a, a, M, BM, CU_TENSOR_MAP_SWIZZLE_NONE) || !encode(&map_b, b, N, BN / 2, CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B))
 			return false;
 		Params p;
 		std::memset(&p, 0, sizeof(p));
@@ -441,7 +521,7 @@ namespace mb200
 		p.k_blocks = k_blocks;
 		p.a_mn = a.mn;
 		p.b_mn = b.mn;
-		p.m_tiles = (M + BM - 1) / BM;
+		p.m_tiles = (M + 2 * BM - 1) / (2 * BM);
 		p.n_tiles = (N + BN - 1) / BN;
 		p.blocks_per_split = (k_blocks + splits - 1) / splits;
 		p.splits = splits;
@@ -455,7 +535,20 @@ namespace mb200
 			record_error(ctx, "gemm_fp32: %d x %d tiles are too many for one launch", p.m_tiles, p.n_tiles);
 			return false;
 		}
-		const cudaError_t status = launch_overlapped(kernel_gemm_fp32, dim3(static_cast<unsigned>(std::min<long long>(units, c->sm_count))), dim3(THREADS), SMEM_BYTES, stream, map_a, map_b, p);
+		cudaLaunchConfig_t config = { };
+		cudaLaunchAttribute attributes[2] = { };
+		attributes[0].id = cudaLaunchAttributeClusterDimension;
+		attributes[0].val.clusterDim.x = 2;
+		attributes[0].val.clusterDim.y = attributes[0].val.clusterDim.z = 1;
+		attributes[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+		attributes[1].val.programmaticStreamSerializationAllowed = 1;
+		config.gridDim = dim3(2 * static_cast<unsigned>(std::min<long long>(units, resident)));
+		config.blockDim = dim3(THREADS);
+		config.dynamicSmemBytes = SMEM_BYTES;
+		config.stream = use_stream(ctx);
+		config.attrs = attributes;
+		config.numAttrs = 2;
+		const cudaError_t status = cudaLaunchKernelEx(&config, kernel_gemm_fp32, map_a, map_b, p);
 		MB200_COUNT_LAUNCH();
 		c->kernels_with_waits = true;
 		if (!check_cuda(ctx, status, "gemm_fp32 launch"))

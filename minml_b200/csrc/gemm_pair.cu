@@ -126,12 +126,6 @@ namespace mb200
 			return kept + static_cast<long long>(row0) * 2 * p.N + static_cast<long long>(column) * min(32, p.M - row0);
 		}
 
-		/* On the even CTA's barrier.  What it reports is that tensor memory has been read (ordered by tcgen05.fence), no memory write: a release at
-		 * cluster scope would wait for every store of the thread, measured as the largest stall of the short-K epilogues. */
-		__device__ __forceinline__ void arrive_at_leader(uint32_t bar)
-		{
-			asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" :: "r"(map_to_cta(bar, 0)) : "memory");
-		}
 
 		/* A warp's 32 x 32 boxes in shared memory: a lane owns one row.  fp16: 64-byte rows, 16-byte piece k at k ^ (row / 2 % 4) (64-byte
 		 * swizzle); fp32: 128-byte rows, piece k at k ^ (row % 8) (128-byte swizzle). */

@@ -333,6 +333,12 @@ namespace mb200
 		{
 			asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" :: "r"(bar) : "memory");
 		}
+		/* On the even CTA's barrier.  What it reports is that tensor memory has been read (ordered by tcgen05.fence), no memory write: a release at
+		 * cluster scope would wait for every store of the thread, measured as the largest stall of the short-K epilogues. */
+		__device__ __forceinline__ void arrive_at_leader(uint32_t bar)
+		{
+			asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" :: "r"(map_to_cta(bar, 0)) : "memory");
+		}
 		__device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t parity)
 		{
 			uint32_t done;
@@ -390,6 +396,16 @@ namespace mb200
 						"tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t"
 						"}\n" :: "r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
 		}
+		/* A in the tensor memory of both CTAs (at the same columns: one 32-bit element a column, a row of the CTA's half a lane) */
+		__device__ __forceinline__ void mma_ts_tf32_pair(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate)
+		{
+			asm volatile(
+					"{\n\t"
+					".reg .pred p;\n\t"
+					"setp.ne.b32 p, %4, 0;\n\t"
+					"tcgen05.mma.cta_group::2.kind::tf32 [%0], [%1], %2, %3, p;\n\t"
+					"}\n" :: "r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
+		}
 		/* One arrival on the barrier at this shared-memory offset in BOTH CTAs of the pair, once every tcgen05.mma issued so
 		 * far by this thread has completed.  (A barrier arrival, not a data load.) */
 		__device__ __forceinline__ void mma_commit_pair(uint32_t bar)
@@ -401,6 +417,10 @@ namespace mb200
 		__host__ __device__ constexpr uint32_t make_idesc_f16_pair(int n)
 		{
 			return (1u << 4) | (0u << 7) | (0u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(256 >> 4) << 24);
+		}
+		__host__ __device__ constexpr uint32_t make_idesc_tf32_pair(int n)
+		{
+			return (1u << 4) | (2u << 7) | (2u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(256 >> 4) << 24);
 		}
 		__host__ __device__ constexpr uint32_t make_idesc_i8_pair(int n)
 		{
