@@ -50,8 +50,10 @@ namespace mb200
 				int M, N, k_blocks;
 				int a_mn, b_mn;
 				int m_tiles, n_tiles, splits, blocks_per_split;
-				float *d; // splits > 1: [splits, M, ldd] sums
+				float *d; // splits > 1: sums of each K range, split_stride elements apart
 				int ldd;
+				long long split_stride;
+				int transposed; // d [N, ldd] takes the transpose
 				float beta;
 				int *status;
 		};
@@ -336,6 +338,20 @@ namespace mb200
 					}
 					if (!ok)
 						break;
+					float *d = p.d + u.split * p.split_stride;
+					if (p.transposed)
+					{ // a column's 32 rows are 128 contiguous bytes
+						const int m = u.m0 + q * 32 + lane, n = u.n0 + half * (BN / 2), columns = min(BN / 2, p.N - n);
+						if (m < p.M)
+						{
+							float *dst = d + static_cast<long long>(n) * p.ldd + m;
+#pragma unroll
+							for (int j = 0; j < BN / 2; j++, dst += p.ldd)
+								if (j < columns)
+									*dst = p.beta != 0.0f ? v[j] + p.beta * *dst : v[j];
+						}
+						continue;
+					}
 					// a lane holds 64 columns of one row; through shared memory, so that a store instruction covers 128 bytes of one row
 					const int row0 = u.m0 + q * 32, rows = min(32, p.M - row0);
 					const uint32_t box = lo_base + LO_STAGES * B_BYTES + (warp - EPI_FIRST) * BOX_BYTES;
@@ -350,7 +366,7 @@ namespace mb200
 						__syncwarp();
 						if (n < p.N)
 						{
-							float *dst = p.d + (static_cast<long long>(u.split) * p.M + row0) * p.ldd + n;
+							float *dst = d + static_cast<long long>(row0) * p.ldd + n;
 #pragma unroll 8
 							for (int r = 0; r < rows; r++, dst += p.ldd)
 							{
@@ -458,10 +474,19 @@ namespace mb200
 			}
 			return std::max(0, known[device]);
 		}
+		/* Tiles of 256 x 128; the product's transpose, where it has fewer (300 rows are 384 as columns, 512 as rows). */
+		long long tiles_of(int M, int N)
+		{
+			return static_cast<long long>((M + 2 * BM - 1) / (2 * BM)) * ((N + BN - 1) / BN);
+		}
+		bool takes_transpose(int M, int N)
+		{
+			return tiles_of(N, M) < tiles_of(M, N);
+		}
 		int float_splits(mlContext_t ctx, int M, int N, int K)
 		{
 			const int clusters = std::max(1, resident_clusters(ctx));
-			const long long tiles = static_cast<long long>((M + 2 * BM - 1) / (2 * BM)) * ((N + BN - 1) / BN);
+			const long long tiles = std::min(tiles_of(M, N), tiles_of(N, M));
 			const int k_blocks = (K + BK - 1) / BK;
 			int best = 1;
 			double best_time = 0.0;
@@ -510,23 +535,28 @@ namespace mb200
 			const uint32_t box[3] = { 32, o.mn ? 32u : box_rows, 1 };
 			return encode_tensor_map(ctx, map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, o.data, dims, strides, box, o.mn ? swizzle_mn : CU_TENSOR_MAP_SWIZZLE_128B);
 		};
+		const bool transposed = takes_transpose(M, N);
+		const FloatOperand &first = transposed ? b : a, &second = transposed ? a : b;
+		const int rows = transposed ? N : M, columns = transposed ? M : N; // of what the kernel multiplies
 		CUtensorMap map_a, map_b;
-		if (!encode(&map_a, a, M, BM, CU_TENSOR_MAP_SWIZZLE_NONE) || !encode(&map_b, b, N, BN / 2, CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B))
+		if (!encode(&map_a, first, rows, BM, CU_TENSOR_MAP_SWIZZLE_NONE) || !encode(&map_b, second, columns, BN / 2, CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B))
 			return false;
 		Params p;
 		std::memset(&p, 0, sizeof(p));
 		const int splits = float_splits(ctx, M, N, K), k_blocks = (K + BK - 1) / BK;
-		p.M = M;
-		p.N = N;
+		p.M = rows;
+		p.N = columns;
+		p.transposed = transposed;
 		p.k_blocks = k_blocks;
-		p.a_mn = a.mn;
-		p.b_mn = b.mn;
-		p.m_tiles = (M + 2 * BM - 1) / (2 * BM);
-		p.n_tiles = (N + BN - 1) / BN;
+		p.a_mn = first.mn;
+		p.b_mn = second.mn;
+		p.m_tiles = (rows + 2 * BM - 1) / (2 * BM);
+		p.n_tiles = (columns + BN - 1) / BN;
 		p.blocks_per_split = (k_blocks + splits - 1) / splits;
 		p.splits = splits;
 		p.d = splits > 1 ? partials : d;
 		p.ldd = splits > 1 ? partial_pitch(N) : ldd;
+		p.split_stride = static_cast<long long>(M) * p.ldd;
 		p.beta = splits > 1 ? 0.0f : beta;
 		p.status = c->dev_status;
 		const long long units = static_cast<long long>(p.m_tiles) * p.n_tiles * splits;
