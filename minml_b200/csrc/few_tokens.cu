@@ -88,10 +88,6 @@ namespace mb200
 			asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
 			return v;
 		}
-		__device__ __forceinline__ void st_shared_f32(uint32_t addr, float v)
-		{
-			asm volatile("st.shared.f32 [%0], %1;" :: "r"(addr), "f"(v) : "memory");
-		}
 
 		__device__ __forceinline__ float warp_max(float v)
 		{ // of all lanes, in every lane; a NaN gives way to a number

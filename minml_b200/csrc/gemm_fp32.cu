@@ -32,7 +32,7 @@ namespace mb200
 		constexpr int BM = 128, BN = 128, BK = 32;
 		constexpr int A_BYTES = BM * BK * 4, B_BYTES = BN / 2 * BK * 4; // of a CTA
 		constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-		constexpr int STAGES = 6, LO_STAGES = 4, BUFFERS = 2;
+		constexpr int STAGES = 5, LO_STAGES = 4, BUFFERS = 2;
 		constexpr int A_COLUMNS = 2 * BK; // of tensor memory: hi and lo of a stage of A, a row a lane
 		constexpr int TMEM_COLUMNS = 512;
 		static_assert(BUFFERS * BN + LO_STAGES * A_COLUMNS <= TMEM_COLUMNS, "tensor memory");
@@ -42,8 +42,8 @@ namespace mb200
 		constexpr int REGISTERS_FEW = 40, REGISTERS_EPILOGUE = 144, REGISTERS_SPLIT = 72;
 		static_assert(128 * REGISTERS_FEW + 256 * REGISTERS_EPILOGUE + 256 * REGISTERS_SPLIT <= THREADS * 96, "registers of the block at launch");
 		constexpr int BOX_MN_BYTES = BK * 128; // 32 rows of an operand that is stored [K, rows]
-		constexpr int BOX_BYTES = 32 * 128; // per epilogue warp: 32 x 32 results
-		constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + LO_STAGES * B_BYTES + EPI_WARPS * BOX_BYTES + 1024;
+		constexpr int BOX_BYTES = 32 * 128; // 32 x 32 results, two an epilogue warp
+		constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + LO_STAGES * B_BYTES + EPI_WARPS * 2 * BOX_BYTES + 1024;
 
 		struct Params
 		{
@@ -54,6 +54,7 @@ namespace mb200
 				int ldd;
 				long long split_stride;
 				int transposed; // d [N, ldd] takes the transpose
+				int by_copies; // d is stored through map_d
 				float beta;
 				int *status;
 		};
@@ -72,7 +73,8 @@ namespace mb200
 			return (__float_as_uint(lo) + 0x1000u) & 0xFFFFE000u;
 		}
 
-		__global__ void __launch_bounds__(THREADS, 1) kernel_gemm_fp32(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Params p)
+		__global__ void __launch_bounds__(THREADS, 1) kernel_gemm_fp32(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+				const __grid_constant__ CUtensorMap map_d, const Params p)
 		{
 			extern __shared__ uint8_t smem_raw[];
 			__shared__ Barriers bars;
@@ -302,6 +304,7 @@ namespace mb200
 			{ /* ------------------------------------------------------------ sums and results */
 				asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(REGISTERS_EPILOGUE));
 				const int q = warp % 4, half = (warp - EPI_FIRST) / 4;
+				const uint32_t boxes = lo_base + LO_STAGES * B_BYTES + (warp - EPI_FIRST) * 2 * BOX_BYTES;
 				uint32_t it = 0;
 				bool ok = true;
 				for (int unit = first_unit; unit < units && ok; unit += unit_step)
@@ -338,35 +341,44 @@ namespace mb200
 					}
 					if (!ok)
 						break;
-					float *d = p.d + u.split * p.split_stride;
-					if (p.transposed)
-					{ // a column's 32 rows are 128 contiguous bytes
-						const int m = u.m0 + q * 32 + lane, n = u.n0 + half * (BN / 2), columns = min(BN / 2, p.N - n);
-						if (m < p.M)
-						{
-							float *dst = d + static_cast<long long>(n) * p.ldd + m;
-#pragma unroll
-							for (int j = 0; j < BN / 2; j++, dst += p.ldd)
-								if (j < columns)
-									*dst = p.beta != 0.0f ? v[j] + p.beta * *dst : v[j];
-						}
-						continue;
-					}
-					// a lane holds 64 columns of one row; through shared memory, so that a store instruction covers 128 bytes of one row
-					const int row0 = u.m0 + q * 32, rows = min(32, p.M - row0);
-					const uint32_t box = lo_base + LO_STAGES * B_BYTES + (warp - EPI_FIRST) * BOX_BYTES;
+					// a lane holds 64 columns of one row: to boxes of 32 x 32 of the result, which the copy engine stores while the next tile is summed
+					// up, or, where it cannot (beta, alignment), the warp stores 128 bytes of a row at a time
+					const int result_rows = p.transposed ? p.N : p.M, result_columns = p.transposed ? p.M : p.N;
+					if (lane == 0)
+						bulk_wait_group_read<0>(); // of the last tile's boxes
+					__syncwarp();
 #pragma unroll
 					for (int c = 0; c < 2; c++)
 					{
-						const int n = u.n0 + half * (BN / 2) + c * 32 + lane;
-#pragma unroll
-						for (int k = 0; k < 8; k++)
-							st_shared_v4(box + lane * 128 + ((k ^ (lane & 7)) * 16), make_uint4(__float_as_uint(v[c * 32 + 4 * k]), __float_as_uint(v[c * 32 + 4 * k + 1]),
-									__float_as_uint(v[c * 32 + 4 * k + 2]), __float_as_uint(v[c * 32 + 4 * k + 3])));
-						__syncwarp();
-						if (n < p.N)
+						const uint32_t box = boxes + c * BOX_BYTES;
+						const int along_m = u.m0 + q * 32, along_n = u.n0 + half * (BN / 2) + c * 32;
+						const int row0 = p.transposed ? along_n : along_m, column0 = p.transposed ? along_m : along_n;
+						if (p.transposed)
 						{
-							float *dst = d + static_cast<long long>(row0) * p.ldd + n;
+#pragma unroll
+							for (int j = 0; j < 32; j++)
+								st_shared_f32(box + j * 128 + (((lane / 4) ^ (j & 7)) * 16) + lane % 4 * 4, v[c * 32 + j]);
+						}
+						else
+						{
+#pragma unroll
+							for (int k = 0; k < 8; k++)
+								st_shared_v4(box + lane * 128 + ((k ^ (lane & 7)) * 16), make_uint4(__float_as_uint(v[c * 32 + 4 * k]), __float_as_uint(v[c * 32 + 4 * k + 1]),
+										__float_as_uint(v[c * 32 + 4 * k + 2]), __float_as_uint(v[c * 32 + 4 * k + 3])));
+						}
+						if (p.by_copies)
+						{
+							fence_proxy_async_smem();
+							__syncwarp();
+							if (lane == 0 && row0 < result_rows && column0 < result_columns)
+								tma_store_3d(&map_d, box, column0, row0, u.split);
+							continue;
+						}
+						__syncwarp();
+						const int rows = min(32, result_rows - row0), column = column0 + lane;
+						if (column < result_columns)
+						{
+							float *dst = p.d + u.split * p.split_stride + static_cast<long long>(row0) * p.ldd + column;
 #pragma unroll 8
 							for (int r = 0; r < rows; r++, dst += p.ldd)
 							{
@@ -374,9 +386,13 @@ namespace mb200
 								*dst = p.beta != 0.0f ? x + p.beta * *dst : x;
 							}
 						}
-						__syncwarp();
 					}
+					if (lane == 0)
+						bulk_commit_group();
 				}
+				if (lane == 0)
+					bulk_wait_group_read<0>(); // shared memory stays until the last store has read it
+				__syncwarp();
 			}
 
 			tcgen05_fence_before();
@@ -559,6 +575,16 @@ namespace mb200
 		p.split_stride = static_cast<long long>(M) * p.ldd;
 		p.beta = splits > 1 ? 0.0f : beta;
 		p.status = c->dev_status;
+		CUtensorMap map_d = map_a; // unused unless by_copies
+		p.by_copies = p.beta == 0.0f && p.ldd % 4 == 0 && aligned_to(p.d, 16);
+		if (p.by_copies)
+		{
+			const uint64_t dims[3] = { static_cast<uint64_t>(N), static_cast<uint64_t>(M), static_cast<uint64_t>(splits) };
+			const uint64_t strides[2] = { static_cast<uint64_t>(p.ldd) * 4, static_cast<uint64_t>(p.split_stride) * 4 };
+			const uint32_t box[3] = { 32, 32, 1 };
+			if (!encode_tensor_map(ctx, &map_d, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, p.d, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B))
+				return false;
+		}
 		const long long units = static_cast<long long>(p.m_tiles) * p.n_tiles * splits;
 		if (units > 0x3FFFFFFF)
 		{
@@ -578,7 +604,7 @@ namespace mb200
 		config.stream = use_stream(ctx);
 		config.attrs = attributes;
 		config.numAttrs = 2;
-		const cudaError_t status = cudaLaunchKernelEx(&config, kernel_gemm_fp32, map_a, map_b, p);
+		const cudaError_t status = cudaLaunchKernelEx(&config, kernel_gemm_fp32, map_a, map_b, map_d, p);
 		MB200_COUNT_LAUNCH();
 		c->kernels_with_waits = true;
 		if (!check_cuda(ctx, status, "gemm_fp32 launch"))

@@ -514,6 +514,10 @@ namespace mb200
 			asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
 			return d;
 		}
+		__device__ __forceinline__ void st_shared_f32(uint32_t addr, float v)
+		{
+			asm volatile("st.shared.f32 [%0], %1;" :: "r"(addr), "f"(v) : "memory");
+		}
 		__device__ __forceinline__ float ld_shared_f32(uint32_t addr)
 		{
 			float v;
