@@ -1,15 +1,20 @@
 /*
  * gemm_fp32.cu -- fp32 matrix products that keep fp32 accuracy at any K, on the TF32 tensor cores.
  *
- * Every element is split into hi, its upper 19 bits, which is what the tensor core reads of the fp32 tile as it lies in shared memory, and
- * lo = x - hi rounded to TF32, which warps write to a tile of their own; hi hi + hi lo + lo hi is accumulated.  Dropped are lo lo, at most
- * 2^-20 of the product and 2^-22 on average, and lo's rounding, 2^-21.  But the tensor core cuts its sums instead of rounding them, measured
- * 2e-8 of the sum for every 8 K indices and product, always toward zero: 3.7e-6 at K = 512 and 5.7e-5 at K = 8192, where an fp32 sum is off
- * by 4e-7 and 7e-7.  So an accumulator here takes one stage, 32 K indices (12 instructions, 2.3e-7), and the epilogue warps add it to sums that
- * they hold in registers, 64 columns a lane; four accumulators in tensor memory keep the tensor core ahead of them.
- * One CTA per SM, persistent over 128 x 128 tiles and, where there are few tiles, K ranges whose sums a second kernel adds up:
- *   warp 0 TMA, warp 1 multiplications, warps 2-9 sums and results, warps 10-13 split.
- * Shared-memory bandwidth bounds it (a stage is read and written by the copy, the split and three products).
+ * Every element is split into hi, its upper 19 bits, which is what the tensor core reads of an fp32 value, and lo = x - hi rounded to TF32;
+ * hi hi + hi lo + lo hi is accumulated.  Dropped are lo lo, at most 2^-20 of the product and 2^-22 on average, and lo's rounding, 2^-21.  But the
+ * tensor core cuts its sums instead of rounding them, measured 2e-8 of the sum for every 8 K indices and product, always toward zero:
+ * 3.7e-6 at K = 512 and 5.7e-5 at K = 8192, where an fp32 sum is off by 4e-7 and 7e-7.  So an accumulator here takes one stage, 32 K indices
+ * (12 instructions, 2.3e-7), and the epilogue warps add it to sums that they hold in registers, 64 columns a lane.
+ * A cluster of two CTAs computes 256 x 128 tiles (cta_group::2), persistent over tiles and, where there are few, K ranges whose sums a second
+ * kernel adds up.  Where the transposed product has fewer tiles, it is the one computed, and stored transposed.
+ *   warp 0 TMA, warp 1 multiplications (of the even CTA), warps 4-11 sums and results, warps 12-19 split, two groups that take stages in turn.
+ * Shared memory would bound it: with one CTA a tile and both terms of both operands there, a stage took 1400 cycles for 770 of
+ * multiplications.  So A's terms go to tensor memory (a lane a row, 64 columns a stage; as a side effect it does not matter how A is stored),
+ * each CTA holds and splits half of B, and of B's hi the tile that TMA wrote serves.  What bounded it next was the time from a tile's arrival
+ * to its split, 700 cycles of one group of warps (two: 2504 -> 2115 us below), of which an arrival with release at cluster scope would
+ * take 950 more.  Now the tensor core is busy 84 % of the time at 1.44 GHz, the clock under the power limit (4096 x 4096 x 8192).
+ * Measured, gated block forward and backward, 2000 x 4001 x 3001: 2085 us (3191 with one CTA a tile), 8192 x 2048 x 8192: 11.0 ms, 225 TFLOP/s.
  */
 #include "common.cuh"
 #include "tc.cuh"
@@ -454,7 +459,7 @@ namespace mb200
 	template bool pack_rows<__half>(mlContext_t, __half*, int, long long, const __half*, long long, int, int);
 	template bool pack_rows<float>(mlContext_t, float*, int, long long, const float*, long long, int, int);
 
-	/* As pair_splits (gemm_pair.cu), with this kernel's figures: a K block of a tile 0.75 us. */
+	/* As pair_splits (gemm_pair.cu), with this kernel's figures: a K block of a tile 0.5 us. */
 	namespace
 	{
 		/* How many clusters the device holds at once; 0 when they cannot be placed.  Also opts the kernel in to its shared memory; both once per device. */
