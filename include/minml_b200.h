@@ -296,8 +296,10 @@ void mb200_convolution_forward_noalloc(mlContext_t context, mlDataType_t dtype, 
  * is the caller's: mb200_*_get_workspace_size tells how much, `workspace` is a descriptor of at least that many bytes, 16-byte aligned,
  * whose contents need not survive between calls; calls that may overlap on the GPU (two contexts, two replayed graphs) need one each.
  * fp16 and fp32 matrices whose row length is a multiple of 16 bytes must be 16-byte aligned (where they are operands of a product), others
- * are copied to padded rows in the workspace first.  No call allocates or synchronises, so each may be captured into a CUDA graph.  Results do not depend on timing (no atomics in sums):
- * the same call gives the same bits. */
+ * are copied to padded rows in the workspace first or, by a forward pass over a few rows, read in place.  No call allocates or synchronises,
+ * so each may be captured into a CUDA graph.  Results do not depend on timing (no atomics in sums): the same call gives the same bits.
+ * fp32 products split their operands (error about that of an fp32 sum): an infinite element may give NaN where fp32 arithmetic gives an
+ * infinity. */
 
 /* Layer normalisation that keeps what its backward pass needs: y as cuda_layernorm_forward, stats [rows, 2] fp32 = (mean, 1 / stddev) of
  * x + ext.  ext, w, b are optional.  y may be x or ext itself for rows of up to 8192 channels. */
