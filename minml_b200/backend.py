@@ -368,23 +368,29 @@ def activationBackward(ctx, dy, y, dx, act="linear", alpha=1.0, beta=0.0):
 
 # ---------------------------------------------------------------------------------------------- training and serving of transformer blocks
 # (extensions: the reference has no counterpart; the C declarations in include/minml_b200.h say what each argument means)
-def _operand(t, ctx):
-    """desc for the functions below, which refuse what is not a dense tensor on the context's device instead of asserting."""
-    if t is None:
-        return _EMPTY
-    if t.get_device() != ctx.device_index:
-        raise BackendError("tensor on %s passed to a context of cuda:%d" % (t.device, ctx.device_index))
-    shape = t.shape
-    rank = len(shape)
-    if rank > 6 or not t.is_contiguous():
-        raise BackendError("a dense row-major tensor of at most 6 dimensions is needed, not %s with strides %s" % (tuple(shape), t.stride()))
-    return mlTensor_t.from_buffer_copy(_PACK(t.data_ptr(), _DTYPES.get(t.dtype, _abi.DTYPE_UNKNOWN), rank, *shape, *_FILL[rank]))
+def _refuse(t, device_index):
+    if t.get_device() != device_index:
+        raise BackendError("tensor on %s passed to a context of cuda:%d" % (t.device, device_index))
+    raise BackendError("a dense row-major tensor of at most 6 dimensions is needed, not %s with strides %s" % (tuple(t.shape), t.stride()))
+
+
+def _load_binding():
+    """The functions below describe up to nine tensors a call, which an extension module does in a fraction of the time (csrc/binding.c)."""
+    try:
+        from . import _binding
+    except ImportError as e:
+        raise RuntimeError("minml_b200/_binding.so is missing or does not load (%s): run `python -m minml_b200.build`" % e)
+    names = [name for name in _abi.declared_symbols() if name.startswith("mb200_")]
+    _binding.bind({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in names}, _DTYPES, _refuse, BackendError)
+    return _binding
+
+
+_binding = _load_binding()
 
 
 def layernormForwardTraining(ctx, x, y, weights, bias, stats, ext=None):
     """layernormForward that also writes stats (fp32 [rows, 2]: mean and 1 / stddev of every row) for layernormBackward."""
-    lib.mb200_layernorm_forward(ctx.handle, _operand(x, ctx), _operand(ext, ctx), _operand(weights, ctx), _operand(bias, ctx), _operand(y, ctx), _operand(stats, ctx))
-    ctx.check()
+    _binding.layernorm_forward(ctx.handle, ctx.device_index, x, ext, weights, bias, y, stats)
 
 
 def layernormBackwardGetWorkspaceSize(ctx, x_shape):
@@ -394,9 +400,7 @@ def layernormBackwardGetWorkspaceSize(ctx, x_shape):
 
 def layernormBackward(ctx, x, dy, dx, weights, stats, dw=None, db=None, ext=None, beta_dx=0.0, beta_dw=0.0, workspace=None):
     """dx = gradient of x (and of ext) + beta_dx * dx; dw, db (fp32 or x's type) = gradients + beta_dw * old values, reduced in a fixed order."""
-    lib.mb200_layernorm_backward(ctx.handle, _operand(x, ctx), _operand(ext, ctx), _operand(dy, ctx), _operand(weights, ctx), _operand(stats, ctx), beta_dx, _operand(dx, ctx), beta_dw,
-                                 _operand(dw, ctx), _operand(db, ctx), _operand(workspace, ctx))
-    ctx.check()
+    _binding.layernorm_backward(ctx.handle, ctx.device_index, x, ext, dy, weights, stats, dx, dw, db, workspace, beta_dx, beta_dw)
 
 
 GATES = {"sigmoid": 0, "relu": 1, "silu": 2, "gelu": 3}
@@ -421,15 +425,12 @@ def gatedFeedForwardGetWorkspaceSize(ctx, x_shape, w1_shape, dtype=torch.float16
 
 def gatedFeedForwardForward(ctx, x, w1, w2, y, gate="silu", beta=0.0, saved=None, workspace=None):
     """y = (act(x Wg^T) * (x Wu^T)) W2^T + beta * y, w1 = [Wg; Wu] of shape [2 hidden, embed], w2 of shape [embed, hidden]."""
-    lib.mb200_gated_feed_forward_forward(ctx.handle, _operand(x, ctx), _operand(w1, ctx), _operand(w2, ctx), beta, _operand(y, ctx), gate_code(gate), _operand(saved, ctx), _operand(workspace, ctx))
-    ctx.check()
+    _binding.gated_feed_forward_forward(ctx.handle, ctx.device_index, x, w1, w2, y, saved, workspace, beta, gate_code(gate))
 
 
 def gatedFeedForwardBackward(ctx, x, w1, w2, dy, dx=None, dw1=None, dw2=None, gate="silu", saved=None, beta_dx=0.0, beta_dw=0.0, workspace=None):
     """Gradients of gatedFeedForwardForward for dy; `saved` is the tensor given to the forward call, or None (then it is computed again)."""
-    lib.mb200_gated_feed_forward_backward(ctx.handle, _operand(x, ctx), _operand(w1, ctx), _operand(w2, ctx), _operand(saved, ctx), _operand(dy, ctx), beta_dx, _operand(dx, ctx), beta_dw,
-                                          _operand(dw1, ctx), _operand(dw2, ctx), gate_code(gate), _operand(workspace, ctx))
-    ctx.check()
+    _binding.gated_feed_forward_backward(ctx.handle, ctx.device_index, x, w1, w2, saved, dy, dx, dw1, dw2, workspace, beta_dx, beta_dw, gate_code(gate))
 
 
 def softmaxCrossEntropyGetWorkspaceSize(ctx, x_shape, w_shape, dtype=torch.float16, training=False):
@@ -438,12 +439,9 @@ def softmaxCrossEntropyGetWorkspaceSize(ctx, x_shape, w_shape, dtype=torch.float
 
 def softmaxCrossEntropyForward(ctx, x, weights, targets, loss, lse=None, workspace=None):
     """loss[t] = log sum_v exp(x_t . w_v) - x_t . w_target (fp32), 0 for a target outside the vocabulary; lse[t] keeps the first term."""
-    lib.mb200_softmax_cross_entropy_forward(ctx.handle, _operand(x, ctx), _operand(weights, ctx), _operand(targets, ctx), _operand(loss, ctx), _operand(lse, ctx), _operand(workspace, ctx))
-    ctx.check()
+    _binding.softmax_cross_entropy_forward(ctx.handle, ctx.device_index, x, weights, targets, loss, lse, workspace)
 
 
 def softmaxCrossEntropyBackward(ctx, x, weights, targets, lse, dx=None, dw=None, alpha=1.0, row_weights=None, beta_dx=0.0, beta_dw=0.0, workspace=None):
     """Gradients of alpha * sum_t row_weights[t] * loss[t], each + beta times its old value."""
-    lib.mb200_softmax_cross_entropy_backward(ctx.handle, _operand(x, ctx), _operand(weights, ctx), _operand(targets, ctx), _operand(lse, ctx), alpha, _operand(row_weights, ctx), beta_dx, _operand(dx, ctx),
-                                             beta_dw, _operand(dw, ctx), _operand(workspace, ctx))
-    ctx.check()
+    _binding.softmax_cross_entropy_backward(ctx.handle, ctx.device_index, x, weights, targets, lse, row_weights, dx, dw, workspace, alpha, beta_dx, beta_dw)

@@ -3,7 +3,7 @@
 Usage:  python -m minml_b200.build [--force] [--verbose]
 
 Each .cu file under minml_b200/csrc is compiled to an object file (in parallel) and the objects are linked into
-minml_b200/libminml_b200.so.  Objects are rebuilt only when their source or a header is newer.  The library links
+minml_b200/libminml_b200.so, and csrc/binding.c to the extension module minml_b200/_binding.so.  Objects are rebuilt only when their source or a header is newer.  The library links
 the CUDA runtime statically and fetches the one driver entry point it needs (cuTensorMapEncodeTiled) at run time,
 so it has no link-time dependency on libcuda.
 """
@@ -11,12 +11,15 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 ROOT = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(ROOT, "csrc")
 OBJ = os.path.join(ROOT, "build")
 LIB = os.path.join(ROOT, "libminml_b200.so")
+BINDING = os.path.join(ROOT, "_binding.so")
+HEADER = os.path.join(ROOT, "..", "include", "minml_b200.h")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
@@ -33,8 +36,19 @@ def find_nvcc():
 
 def _newest_header():
     times = [os.path.getmtime(os.path.join(CSRC, f)) for f in os.listdir(CSRC) if f.endswith((".cuh", ".h"))]
-    times.append(os.path.getmtime(os.path.join(ROOT, "..", "include", "minml_b200.h")))
+    times.append(os.path.getmtime(HEADER))
     return max(times)
+
+
+def build_binding(force=False):
+    """The extension module is plain C against Python.h and takes the library's functions by address, so it links with nothing."""
+    source = os.path.join(CSRC, "binding.c")
+    if force or not os.path.exists(BINDING) or os.path.getmtime(BINDING) < max(os.path.getmtime(source), os.path.getmtime(HEADER)):
+        cmd = [os.environ.get("CC") or "gcc", "-O2", "-Wall", "-shared", "-fPIC", "-I", sysconfig.get_paths()["include"], "-I", os.path.dirname(HEADER), "-o", BINDING, source]
+        proc = subprocess.run(cmd, capture_output=True, text=True)
+        if proc.returncode != 0:
+            raise RuntimeError("building the extension module failed:\n%s\n%s" % (proc.stdout, proc.stderr))
+    return BINDING
 
 
 def build(force=False, verbose=False):
@@ -72,6 +86,7 @@ def build(force=False, verbose=False):
         proc = subprocess.run(cmd, capture_output=True, text=True)
         if proc.returncode != 0:
             raise RuntimeError("link failed:\n%s\n%s" % (proc.stdout, proc.stderr))
+    build_binding(force)
     return LIB
 
 
