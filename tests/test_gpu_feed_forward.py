@@ -146,6 +146,26 @@ def test_few_tokens_of_any_row_length(ctx, dtype, embed, hidden, tokens):
         assert bool((around[0] == 7.0).all()) and bool((around[-1] == 7.0).all())
 
 
+@pytest.mark.parametrize("tokens,embed,hidden,dtype", [(1, 512, 1024, torch.float32), (5, 514, 1031, torch.float32), (16, 256, 512, torch.float32), (40, 256, 1000, torch.float32),
+                                                       (3, 1001, 2000, torch.float16), (2, 512, 1024, torch.float16), (300, 264, 512, torch.float32)])
+def test_calls_in_a_row_see_new_values(ctx, dtype, tokens, embed, hidden):
+    """The same buffers with other contents in every call, launched back to back: no kernel may read what an earlier call left in a cache."""
+    from minml_b200 import backend as B
+    x, w1, w2, _ = make(tokens + embed, tokens, embed, hidden, dtype)
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    inputs = [torch.randn(x.shape, device="cuda", generator=gen).to(dtype) for _ in range(12)]
+    results = [nan_like(x) for _ in inputs]
+    ws = workspace(ctx, x, w1, False)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(ctx.torch_stream()):
+        for i in range(len(inputs)):
+            x.copy_(inputs[i])
+            B.gatedFeedForwardForward(ctx, x, w1, w2, results[i], "gelu", workspace=ws)
+    ctx.synchronize()
+    for i in range(len(inputs)):
+        forward(inputs[i], w1, w2, "gelu")[1].holds(results[i], dtype)
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
 def test_few_tokens_off_their_alignment(ctx, dtype):
     """Padded operands may begin at any element, also where their row length alone would allow wider reads."""
