@@ -459,7 +459,7 @@ namespace mb200
 	template bool pack_rows<__half>(mlContext_t, __half*, int, long long, const __half*, long long, int, int);
 	template bool pack_rows<float>(mlContext_t, float*, int, long long, const float*, long long, int, int);
 
-	/* As pair_splits (gemm_pair.cu), with this kernel's figures: a K block of a tile 0.5 us. */
+	/* As pair_splits (gemm_pair.cu), with this kernel's figures: a K block of a tile 0.6 us, the rest of a tile 2, the second kernel 2 and its traffic. */
 	namespace
 	{
 		/* How many clusters the device holds at once; 0 when they cannot be placed.  Also opts the kernel in to its shared memory; both once per device. */
@@ -519,7 +519,7 @@ namespace mb200
 				const double partial_bytes = s == 1 ? 0.0 : 8.0 * s * M * N;
 				if (partial_bytes > 2.0 * (size_t(256) << 20))
 					break;
-				const double time = static_cast<double>((tiles * s + clusters - 1) / clusters) * (blocks * 0.5 + 1.5) + (s == 1 ? 0.0 : 4.0 + partial_bytes / 5.0e6);
+				const double time = static_cast<double>((tiles * s + clusters - 1) / clusters) * (blocks * 0.6 + 2.0) + (s == 1 ? 0.0 : 2.0 + partial_bytes / 5.0e6);
 				if (s == 1 || time < best_time)
 				{
 					best = s;
