@@ -294,6 +294,39 @@ def test_same_bits_and_graphs_with_their_own_workspaces(ctx, tokens, embed, hidd
         assert all(torch.equal(a, b) for a, b in zip(s[-1], want))
 
 
+@pytest.mark.parametrize("tokens,embed,hidden", [(1, 512, 1032), (7, 515, 700), (300, 260, 521), (1500, 128, 640)])
+def test_fp32_same_bits_and_graphs_at_the_same_time(ctx, tokens, embed, hidden):
+    """As above for fp32: pairs of CTAs, few rows and joined K ranges of two graphs share the device."""
+    from minml_b200 import backend as B
+    sets, graphs, want = [], [], []
+    for seed in (1, 2):
+        x, w1, w2, dy = make(seed, tokens, embed, hidden, torch.float32)
+        sets.append((x, w1, w2, dy, torch.empty((tokens, 2 * hidden), device="cuda"), workspace(ctx, x, w1, True), [nan_like(t) for t in (x, x, w1, w2)]))
+
+    def both(x, w1, w2, dy, saved, ws, out):
+        B.gatedFeedForwardForward(ctx, x, w1, w2, out[0], "silu", saved=saved, workspace=ws)
+        B.gatedFeedForwardBackward(ctx, x, w1, w2, dy, out[1], out[2], out[3], "silu", saved=saved, workspace=ws)
+    for s in sets:
+        both(*s)
+        ctx.synchronize()
+        want.append([t.clone() for t in s[-1]])
+        for t in s[-1]:
+            t.fill_(float("nan"))
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=ctx.torch_stream()):
+            both(*s)
+        graphs.append(graph)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(4):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for s, w in zip(sets, want):
+        assert all(torch.equal(a, b) for a, b in zip(s[-1], w))
+
+
 def test_refusals(ctx):
     from minml_b200 import backend as B
     x, w1, w2, dy = make(1, 40, 64, 72, torch.float16)
