@@ -16,7 +16,8 @@
  * fp16 runs on gemm_pair.cu (up to 64 rows forward: few_tokens.cu): forward is one product whose epilogue leaves (maximum, sum of
  * exponentials) for every row and group of columns, joined by a second kernel, and the whole vocabulary is one piece; backward makes 2^15 P of a piece in the epilogue of its logits and
  * multiplies it with W and x.  dx is added up over the pieces in fp32.  fp32 keeps one piece's logits.  An embed that is no multiple of 16
- * bytes is copied to padded rows first.
+ * bytes is copied to padded rows first.  Forward, a few rows in fp32, or in fp16 with such an embed, go through few_rows.cu, which leaves the
+ * same statistics as one product and copies nothing.
  */
 #include "common.cuh"
 #include "operands.cuh"

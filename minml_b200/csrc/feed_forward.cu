@@ -9,7 +9,8 @@
  * fp16: two launches forward (gemm_pair.cu): the first product's tile holds 128 gate and the matching 128 up columns, so its epilogue
  * writes h alone; backward four, [da du] and h coming out of the product that makes dh.  h, da, du are rounded to fp16 once, a and u
  * reach the backward pass in fp32 (rounded to fp16 they would double its error).  fp32: five and eight launches, with the gate between.
- * Extents that are no multiple of 16 bytes are copied to padded rows first: F with zero weights, whose h, da and du are zero.
+ * Forward, a few tokens take two launches of few_tokens.cu (fp16) or of few_rows.cu (fp32, and fp16 rows of odd length, in place).  Elsewhere
+ * extents that are no multiple of 16 bytes are copied to padded rows first: F with zero weights, whose h, da and du are zero.
  */
 #include "common.cuh"
 #include "operands.cuh"
