@@ -78,8 +78,8 @@ namespace mb200
 		}
 
 		/* One block a row: joins the piece's columns [first, first + width) into the row's running maximum and sum. */
-		__global__ void __launch_bounds__(256) kernel_piece_statistics(const float *__restrict__ z, int pitch, float2 *__restrict__ running, float *__restrict__ target_logit, Rows rows,
-				long long tokens, int first, int width, bool last, float *__restrict__ loss, float *__restrict__ lse)
+		__global__ void __launch_bounds__(256) kernel_piece_statistics(const float *z, int pitch, float2 *running, float *target_logit, Rows rows,
+				long long tokens, int first, int width, bool last, float *loss, float *lse)
 		{
 			__shared__ float2 scratch[8];
 			wait_for_previous_grid();
@@ -133,7 +133,7 @@ namespace mb200
 		}
 
 		/* z becomes alpha c_t (exp(z - lse) - [target]) for one piece, four columns a thread; rows that take no part are zero */
-		__global__ void __launch_bounds__(256) kernel_piece_gradient(float *__restrict__ z, int pitch, const float *__restrict__ lse, Rows rows, const GridWalk walk, int first, float alpha)
+		__global__ void __launch_bounds__(256) kernel_piece_gradient(float *z, int pitch, const float *lse, Rows rows, const GridWalk walk, int first, float alpha)
 		{
 			wait_for_previous_grid();
 			const long long stride = static_cast<long long>(gridDim.x) * 256;
@@ -190,8 +190,8 @@ namespace mb200
 			}
 		}
 		/* Joins the statistics of a row's groups, parts[t][group]: a block a row. */
-		__global__ void __launch_bounds__(256) kernel_join_statistics(const float2 *__restrict__ parts, int groups, const float *__restrict__ target_logit, Rows rows,
-				float *__restrict__ loss, float *__restrict__ lse)
+		__global__ void __launch_bounds__(256) kernel_join_statistics(const float2 *parts, int groups, const float *target_logit, Rows rows,
+				float *loss, float *lse)
 		{
 			__shared__ float2 scratch[8];
 			const long long t = blockIdx.x;

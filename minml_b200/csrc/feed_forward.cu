@@ -32,7 +32,7 @@ namespace mb200
 		{
 				float v[4];
 		};
-		__device__ __forceinline__ void load_pre_activations(Four &a, Four &u, const float *__restrict__ au, long long token, int column, int up)
+		__device__ __forceinline__ void load_pre_activations(Four &a, Four &u, const float *au, long long token, int column, int up)
 		{
 			const float *src = au + token * 2 * up + column;
 			if (up % 4 == 0)
@@ -49,7 +49,7 @@ namespace mb200
 			}
 		}
 		template<int GATE>
-		__global__ void __launch_bounds__(256) kernel_gate(float *__restrict__ h, const float *__restrict__ au, const GridWalk walk, int hidden, int up)
+		__global__ void __launch_bounds__(256) kernel_gate(float *h, const float *au, const GridWalk walk, int hidden, int up)
 		{
 			let_next_grid_start();
 			wait_for_previous_grid();
@@ -70,7 +70,7 @@ namespace mb200
 		}
 		/* [da du] and h from dh [tokens, hidden] and the pre-activations */
 		template<int GATE>
-		__global__ void __launch_bounds__(256) kernel_gate_backward(float *__restrict__ dau, float *__restrict__ h, const float *__restrict__ dh, const float *__restrict__ au,
+		__global__ void __launch_bounds__(256) kernel_gate_backward(float *dau, float *h, const float *dh, const float *au,
 				const GridWalk walk, int hidden, int up)
 		{
 			let_next_grid_start();

@@ -418,7 +418,7 @@ namespace mb200
 
 		/* Four destination elements a thread (pitch is a multiple of four). */
 		template<typename T>
-		__global__ void __launch_bounds__(256) kernel_pack_rows(T *__restrict__ dst, int pitch, long long padded_rows, const T *__restrict__ src, long long rows, int columns, const GridWalk walk)
+		__global__ void __launch_bounds__(256) kernel_pack_rows(T *dst, int pitch, long long padded_rows, const T *src, long long rows, int columns, const GridWalk walk)
 		{
 			struct alignas(4 * sizeof(T)) Four
 			{

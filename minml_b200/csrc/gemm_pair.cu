@@ -616,8 +616,8 @@ namespace mb200
 							for (int k = 0; k < 8; k++)
 							{
 								const bool inside = row_ok && n + 4 * k < p.N;
-								const float4 ta = inside ? __ldg(reinterpret_cast<const float4*>(src + k * rows * 4)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-								const float4 tb = inside ? __ldg(reinterpret_cast<const float4*>(src + k * rows * 4 + rows * p.N)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+								const float4 ta = inside ? *reinterpret_cast<const float4*>(src + k * rows * 4) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+								const float4 tb = inside ? *reinterpret_cast<const float4*>(src + k * rows * 4 + rows * p.N) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 								a[4 * k] = ta.x, a[4 * k + 1] = ta.y, a[4 * k + 2] = ta.z, a[4 * k + 3] = ta.w;
 								b[4 * k] = tb.x, b[4 * k + 1] = tb.y, b[4 * k + 2] = tb.z, b[4 * k + 3] = tb.w;
 							}
@@ -876,8 +876,8 @@ namespace mb200
 
 		/* One thread a group of VEC columns: the K ranges' sums in order, the factors, one rounding. */
 		template<typename T, int VEC>
-		__global__ void __launch_bounds__(256) kernel_finish_sums(T *d, int ldd, int M, const GridWalk walk, const float *__restrict__ sums, int pitch, int splits, float alpha,
-				const float *__restrict__ alpha_device, const float *__restrict__ row_scale, float beta)
+		__global__ void __launch_bounds__(256) kernel_finish_sums(T *d, int ldd, int M, const GridWalk walk, const float *sums, int pitch, int splits, float alpha,
+				const float *alpha_device, const float *row_scale, float beta)
 		{
 			struct alignas(sizeof(T) * VEC) Out
 			{

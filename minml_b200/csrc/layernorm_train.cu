@@ -949,7 +949,7 @@ namespace mb200
 		/* dw, db = the sum of the partial rows (+ beta * the old value).  A block takes 32 columns of one of the two; its 32 warps add
 		 * every 32nd row and then each other's sums, always in the same order. */
 		template<typename G>
-		__global__ void __launch_bounds__(1024) kernel_layernorm_add_partials(G *dw, G *db, const float *__restrict__ partial, int blocks, int channels, float beta)
+		__global__ void __launch_bounds__(1024) kernel_layernorm_add_partials(G *dw, G *db, const float *partial, int blocks, int channels, float beta)
 		{
 			__shared__ float sums[32][33];
 			G *out = blockIdx.y == 0 ? dw : db;

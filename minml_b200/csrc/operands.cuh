@@ -166,7 +166,9 @@ namespace mb200
 			}
 	};
 	/* Launch whose grid may start before the grid ahead of it in the stream has finished; the kernel calls griddepcontrol.wait
-	 * (wait_for_previous_grid) before it touches anything that grid wrote. */
+	 * (wait_for_previous_grid) before it touches anything that grid wrote, and reads through pointers without __restrict__ and without __ldg:
+	 * both promise memory that nobody writes during the kernel, which is read through a path that is not coherent and may be read ahead of the
+	 * wait. */
 	template<typename ... KArgs, typename ... Args>
 	inline cudaError_t launch_overlapped(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args ... args)
 	{
