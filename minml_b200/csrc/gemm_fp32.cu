@@ -12,8 +12,9 @@
  * Shared memory would bound it: with one CTA a tile and both terms of both operands there, a stage took 1400 cycles for 770 of
  * multiplications.  So A's terms go to tensor memory (a lane a row, 64 columns a stage; as a side effect it does not matter how A is stored),
  * each CTA holds and splits half of B, and of B's hi the tile that TMA wrote serves.  What bounded it next was the time from a tile's arrival
- * to its split, 700 cycles of one group of warps (two: 2504 -> 2115 us below), of which an arrival with release at cluster scope would
- * take 950 more.  Now the tensor core is busy 84 % of the time at 1.44 GHz, the clock under the power limit (4096 x 4096 x 8192).
+ * to its split, 700 cycles of one group of warps (two: 2504 -> 2115 us below).  The even CTA issues multiplications that read the lo of B which
+ * the odd one's warps wrote, so a split stage is reported with a release at cluster scope, of shared memory alone: of all memory it takes 950
+ * cycles more, or 1 200 to 1 400 of a warp that only passes the report on (2205 us -> 2376 below).  Now the tensor core is busy 84 % of the time at 1.44 GHz, the clock under the power limit (4096 x 4096 x 8192).
  * Measured, gated block forward and backward, 2000 x 4001 x 3001: 2085 us (3191 with one CTA a tile), 8192 x 2048 x 8192: 11.0 ms, 225 TFLOP/s.
  */
 #include "common.cuh"
@@ -301,7 +302,7 @@ namespace mb200
 						fence_proxy_async_smem();
 						__syncwarp();
 						if (lane == 0)
-							arrive_at_leader(smem_u32(&bars.split[s]));
+							publish_to_leader(smem_u32(&bars.split[s]));
 					}
 				}
 			}

@@ -333,11 +333,20 @@ namespace mb200
 		{
 			asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" :: "r"(bar) : "memory");
 		}
-		/* On the even CTA's barrier.  What it reports is that tensor memory has been read (ordered by tcgen05.fence), no memory write: a release at
-		 * cluster scope would wait for every store of the thread, measured as the largest stall of the short-K epilogues. */
+		/* On the even CTA's barrier.  For the one report that tensor memory has been read (tcgen05.wait::ld, ordered by tcgen05.fence): it releases at
+		 * CTA scope, so nothing the thread wrote is thereby visible to the other CTA.  A release at cluster scope (mbar_arrive_cluster) waits for
+		 * every store of the thread, measured as the largest stall of the short-K epilogues. */
 		__device__ __forceinline__ void arrive_at_leader(uint32_t bar)
 		{
 			asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" :: "r"(map_to_cta(bar, 0)) : "memory");
+		}
+		/* On the even CTA's barrier, which waits with an acquire at cluster scope: what this warp's lanes have written to their own CTA's shared memory
+		 * (and put behind fence_proxy_async_smem and __syncwarp) is there for the multiplications that the even CTA then issues.  The release covers
+		 * shared memory alone: one over all memory takes 1 200 to 1 400 cycles in the kernel that uses this (gemm_fp32.cu). */
+		__device__ __forceinline__ void publish_to_leader(uint32_t bar)
+		{
+			asm volatile("fence.release.sync_restrict::shared::cta.cluster;" ::: "memory");
+			asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" :: "r"(map_to_cta(bar, 0)) : "memory");
 		}
 		__device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t parity)
 		{

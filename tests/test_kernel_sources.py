@@ -64,3 +64,10 @@ def test_the_rule_sees_what_it_is_about():
     assert [k[0] for k in found] == ["kernel_a", "kernel_b"]
     assert "__restrict__" in found[0][1] and found[0][2].endswith("f({ 1 }); }")
     assert sum(len(list(kernels(source(f)))) for f in FILES) > 60
+
+
+@pytest.mark.parametrize("name", FILES)
+def test_arrivals_without_a_cluster_release_report_no_writes(name):
+    """arrive_at_leader orders nothing that its thread wrote for the other CTA of the pair; it may only say that accumulators have been read."""
+    barriers = re.findall(r"arrive_at_leader\(smem_u32\(&bars\.(\w+)", source(name))
+    assert set(barriers) <= {"tmem_empty", "au_empty"}, barriers
