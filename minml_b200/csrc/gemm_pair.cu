@@ -13,8 +13,9 @@
  * K and row tails are zero-filled by TMA, results are clipped by their tensor maps.
  *
  * The tensor core cuts its fp32 sums where an fp32 addition would round: measured, 1.6e-8 of the sum for every 16 K indices, always toward
- * zero (4.2e-6 at K = 4096).  That is nothing against a result rounded to fp16, but a loss is kept in fp32, so the
- * epilogue that takes row statistics adds up accumulators of 1024 K indices each in registers.
+ * zero (4.2e-6 at K = 4096).  That is nothing against a result rounded to fp16, but a loss is kept in fp32, and where a row is certain P - 1 is
+ * the difference of two numbers near 1.  So both epilogues of logits add up accumulators of 1024 K indices each in registers, in the same order:
+ * the gradient's logits are those that lse was made from, bit for bit.
  */
 #include "common.cuh"
 #include "tc.cuh"
@@ -45,7 +46,7 @@ namespace mb200
 		// of the 168 registers a thread starts with, what the first four warps give up is what the epilogue gets: 128 * 40 + 256 * 232 = 384 * 168
 		constexpr int REGISTERS_FEW = 40, REGISTERS_MANY = 232;
 		constexpr int HALF_BOX = 32 * 64, FLOAT_BOX = 32 * 128;
-		constexpr int STATISTICS_SEGMENT = 1024 / BK; // K blocks per accumulator in the statistics epilogue
+		constexpr int LOGITS_SEGMENT = 1024 / BK; // K blocks per accumulator of a logit
 		constexpr int ROW_GROUP = 8; // tiles of 256 rows that neighbouring clusters share their columns over
 
 		enum Epilogue
@@ -66,7 +67,8 @@ namespace mb200
 				// per epilogue warp: four 32 x 32 boxes of fp16 or two of fp32; GATED_RECOMPUTE: all six boxes of a tile
 				static constexpr int staging_bytes = EPI == GATED_RECOMPUTE ? 6 * 2048 : 8192;
 				static constexpr int stages = EPI == GATED_RECOMPUTE ? 4 : 5;
-				static constexpr bool moves_registers = EPI == GATED || EPI == GATED_RECOMPUTE || EPI == STATISTICS; // they hold 128 accumulators a thread
+				static constexpr bool sums_segments = EPI == STATISTICS || EPI == PROBABILITIES; // the same logits, to the bit
+				static constexpr bool moves_registers = EPI == GATED || EPI == GATED_RECOMPUTE || sums_segments; // they hold 128 accumulators a thread
 				static constexpr int smem_bytes = stages * STAGE_BYTES + EPI_WARPS * staging_bytes + 1024;
 				static_assert(stages <= MAX_STAGES && smem_bytes <= 227 * 1024, "the configuration exceeds the SM");
 		};
@@ -185,7 +187,7 @@ namespace mb200
 				u.kb1 = min(k_blocks, u.kb0 + p.blocks_per_split);
 				return u;
 			};
-			constexpr int SEGMENT = EPI == STATISTICS ? STATISTICS_SEGMENT : 1 << 30;
+			constexpr int SEGMENT = Shape<EPI>::sums_segments ? LOGITS_SEGMENT : 1 << 30;
 
 			if (threadIdx.x == 0)
 			{
@@ -396,6 +398,27 @@ namespace mb200
 					fence_proxy_async_smem();
 					__syncwarp();
 				};
+				auto sum_segments = [&](const Unit &u, float (&v)[BN / 2]) -> bool
+				{ // this lane's 128 columns of its row
+					for (int kb = u.kb0; kb < u.kb1; kb += SEGMENT)
+					{
+						if (!wait_full())
+							return false;
+						const uint32_t taddr = lane_base + (buffers & 1u) * BN + half * (BN / 2);
+#pragma unroll
+						for (int c = 0; c < BN / 64; c++)
+						{
+							uint32_t r[32];
+							tmem_ld_32x32(taddr + c * 32, r);
+							tmem_wait_ld();
+#pragma unroll
+							for (int j = 0; j < 32; j++)
+								v[c * 32 + j] = (kb == u.kb0 ? 0.0f : v[c * 32 + j]) + __uint_as_float(r[j]);
+						}
+						release();
+					}
+					return true;
+				};
 				for (int unit = first_unit; unit < units && ok; unit += unit_step)
 				{
 					const Unit u = locate(unit);
@@ -405,26 +428,7 @@ namespace mb200
 					if constexpr (EPI == STATISTICS)
 					{
 						float v[BN / 2];
-						for (int kb = u.kb0; kb < u.kb1; kb += SEGMENT)
-						{
-							if (!wait_full())
-							{
-								ok = false;
-								break;
-							}
-							const uint32_t taddr = lane_base + (buffers & 1u) * BN + half * (BN / 2);
-#pragma unroll
-							for (int c = 0; c < BN / 64; c++)
-							{
-								uint32_t r[32];
-								tmem_ld_32x32(taddr + c * 32, r);
-								tmem_wait_ld();
-#pragma unroll
-								for (int j = 0; j < 32; j++)
-									v[c * 32 + j] = (kb == u.kb0 ? 0.0f : v[c * 32 + j]) + __uint_as_float(r[j]);
-							}
-							release();
-						}
+						ok = sum_segments(u, v);
 						if (!ok)
 							break;
 						const int n0 = u.nt * BN + half * (BN / 2), valid = p.N - n0;
@@ -451,17 +455,47 @@ namespace mb200
 						continue;
 					}
 
-					// what the row needs, read under the multiplications
-					int target = -1;
-					float shift = 0.0f, scale = 1.0f;
-					bool active = true;
-					if (EPI == PROBABILITIES)
+					if constexpr (EPI == PROBABILITIES)
 					{
-						target = row_ok ? p.targets[row] : -1;
-						active = target >= 0 && target < p.vocab && (p.row_weights == nullptr || p.row_weights[row] != 0.0f);
-						shift = row_ok ? fmaf(p.lse[row], -LOG2E, 15.0f) : 0.0f; // 2^15 exp(z - lse) = 2^(z log2 e + shift)
+						// what the row needs, read under the multiplications
+						int target = row_ok ? p.targets[row] : -1;
+						const bool active = target >= 0 && target < p.vocab && (p.row_weights == nullptr || p.row_weights[row] != 0.0f);
+						const float shift = row_ok ? fmaf(p.lse[row], -LOG2E, 15.0f) : 0.0f; // 2^15 exp(z - lse) = 2^(z log2 e + shift)
 						target = active ? target - p.first : -1;
+						float v[BN / 2];
+						ok = sum_segments(u, v);
+						if (!ok)
+							break;
+#pragma unroll
+						for (int c = 0; c < BN / 64; c++)
+						{
+							const int n = u.nt * BN + half * (BN / 2) + c * 32;
+							if (n >= p.N)
+								break;
+							float x[32];
+#pragma unroll
+							for (int j = 0; j < 32; j++)
+							{
+								const float e = exp2_approx(fmaf(v[c * 32 + j], LOG2E, shift)) - (target == n + j ? 32768.0f : 0.0f);
+								x[j] = active ? e : 0.0f;
+							}
+							if (lane == 0)
+								bulk_wait_group_read<3>();
+							__syncwarp();
+							const uint32_t box = staging + (boxes++ % 4) * HALF_BOX;
+							write_half_box(box, lane, x);
+							publish();
+							if (lane == 0 && row0 < p.M)
+							{
+								tma_store_2d(&map_d, box, n, row0);
+								bulk_commit_group();
+							}
+						}
+						continue;
 					}
+
+					float scale = 1.0f;
+					bool active = true; // read under the multiplications
 					if (EPI == STORE)
 					{
 						scale = p.result.alpha * (p.result.alpha_device != nullptr ? *p.result.alpha_device : 1.0f);
@@ -680,15 +714,6 @@ namespace mb200
 								bulk_commit_group();
 							}
 							continue;
-						}
-						if (EPI == PROBABILITIES)
-						{
-#pragma unroll
-							for (int j = 0; j < 32; j++)
-							{
-								const float x = exp2_approx(fmaf(v[j], LOG2E, shift)) - (target == n + j ? 32768.0f : 0.0f);
-								v[j] = active ? x : 0.0f;
-							}
 						}
 						if (EPI == STORE)
 						{
