@@ -293,8 +293,9 @@ void mb200_convolution_forward_noalloc(mlContext_t context, mlDataType_t dtype, 
  * entropy gradients are declared above as stubs; its host code has no gated block and no loss fused with the output layer).
  * Common to all: fp16 or fp32 data, dense row-major; the leading extents of a matrix argument may be split ([boards, h, w, channels]
  * is a matrix of boards * h * w rows).  A descriptor with null data and rank 0 stands for an absent optional operand.  Scratch memory
- * is the caller's: mb200_*_get_workspace_size tells how much, `workspace` is a descriptor of at least that many bytes, 16-byte aligned,
- * whose contents need not survive between calls; calls that may overlap on the GPU (two contexts, two replayed graphs) need one each.
+ * is the caller's: mb200_*_get_workspace_size tells how much, `workspace` is a descriptor of at least that many bytes, 16-byte aligned, of any shape
+ * (above 2^31 - 1 bytes it takes more than one extent), whose contents need not survive between calls; calls that may overlap on the GPU (two
+ * contexts, two replayed graphs) need one each.
  * fp16 and fp32 matrices whose row length is a multiple of 16 bytes must be 16-byte aligned (where they are operands of a product), others
  * are copied to padded rows in the workspace first or, by a forward pass over a few rows, read in place.  No call allocates or synchronises,
  * so each may be captured into a CUDA graph.  Results do not depend on timing (no atomics in sums): the same call gives the same bits.

@@ -38,7 +38,10 @@ static long ask(PyObject *t, PyObject *method)
 	Py_DECREF(answer);
 	return value == -1 && PyErr_Occurred() ? -2 : value;
 }
-static bool describe(PyObject *t, PyObject *device, mlTensor_t *result)
+/* The shape of scratch memory says nothing but its size, so where an extent passes a descriptor's 32 bits it is described as rows of 256 elements (sizes asked
+ * for are multiples of 256 bytes). */
+#define SCRATCH_ROW 256
+static bool describe(PyObject *t, PyObject *device, mlTensor_t *result, bool scratch)
 {
 	memset(result, 0, sizeof(*result));
 	result->dtype = DTYPE_UNKNOWN;
@@ -57,11 +60,23 @@ static bool describe(PyObject *t, PyObject *device, mlTensor_t *result)
 	if (fits)
 	{
 		result->rank = (int) PyTuple_GET_SIZE(shape);
+		long elements = 1; /* (of a tensor that exists, so the product fits) */
+		bool long_extent = false;
 		for (int i = 0; i < result->rank && fits; i++)
 		{
 			const long extent = PyLong_AsLong(PyTuple_GET_ITEM(shape, i));
-			fits = extent >= 0 && extent <= INT_MAX;
+			fits = extent >= 0 && (extent <= INT_MAX || scratch);
+			long_extent |= extent > INT_MAX;
+			elements *= extent;
 			result->dim[i] = (int) extent;
+		}
+		if (fits && long_extent)
+		{
+			fits = elements / SCRATCH_ROW <= INT_MAX;
+			memset(result->dim, 0, sizeof(result->dim));
+			result->rank = 2;
+			result->dim[0] = (int) (elements / SCRATCH_ROW);
+			result->dim[1] = SCRATCH_ROW;
 		}
 	}
 	Py_DECREF(shape);
@@ -99,7 +114,11 @@ typedef struct
 		mlTensor_t t[9];
 		double number[3];
 } Arguments;
-static bool take(Arguments *a, PyObject *const *args, Py_ssize_t given, int tensors, int numbers)
+enum Last
+{
+	RESULT, SCRATCH
+}; /* what the last tensor is */
+static bool take(Arguments *a, PyObject *const *args, Py_ssize_t given, int tensors, enum Last last, int numbers)
 {
 	if (given != 2 + tensors + numbers)
 	{
@@ -115,7 +134,7 @@ static bool take(Arguments *a, PyObject *const *args, Py_ssize_t given, int tens
 	if (PyErr_Occurred())
 		return false;
 	for (int i = 0; i < tensors; i++)
-		if (!describe(args[2 + i], args[1], &a->t[i]))
+		if (!describe(args[2 + i], args[1], &a->t[i], last == SCRATCH && i == tensors - 1))
 			return false;
 	for (int i = 0; i < numbers; i++)
 	{
@@ -138,7 +157,7 @@ static PyObject* outcome(const Arguments *a)
 static PyObject* layernorm_forward(PyObject *self, PyObject *const *args, Py_ssize_t given)
 {
 	Arguments a;
-	if (!take(&a, args, given, 6, 0))
+	if (!take(&a, args, given, 6, RESULT, 0))
 		return NULL;
 	Py_BEGIN_ALLOW_THREADS
 	library.layernorm_forward(a.context, a.t[0], a.t[1], a.t[2], a.t[3], a.t[4], a.t[5]);
@@ -148,7 +167,7 @@ static PyObject* layernorm_forward(PyObject *self, PyObject *const *args, Py_ssi
 static PyObject* layernorm_backward(PyObject *self, PyObject *const *args, Py_ssize_t given)
 {
 	Arguments a;
-	if (!take(&a, args, given, 9, 2))
+	if (!take(&a, args, given, 9, SCRATCH, 2))
 		return NULL;
 	Py_BEGIN_ALLOW_THREADS
 	library.layernorm_backward(a.context, a.t[0], a.t[1], a.t[2], a.t[3], a.t[4], (float) a.number[0], a.t[5], (float) a.number[1], a.t[6], a.t[7], a.t[8]);
@@ -158,7 +177,7 @@ static PyObject* layernorm_backward(PyObject *self, PyObject *const *args, Py_ss
 static PyObject* gated_feed_forward_forward(PyObject *self, PyObject *const *args, Py_ssize_t given)
 {
 	Arguments a;
-	if (!take(&a, args, given, 6, 2))
+	if (!take(&a, args, given, 6, SCRATCH, 2))
 		return NULL;
 	Py_BEGIN_ALLOW_THREADS
 	library.gated_feed_forward_forward(a.context, a.t[0], a.t[1], a.t[2], (float) a.number[0], a.t[3], (int) a.number[1], a.t[4], a.t[5]);
@@ -168,7 +187,7 @@ static PyObject* gated_feed_forward_forward(PyObject *self, PyObject *const *arg
 static PyObject* gated_feed_forward_backward(PyObject *self, PyObject *const *args, Py_ssize_t given)
 {
 	Arguments a;
-	if (!take(&a, args, given, 9, 3))
+	if (!take(&a, args, given, 9, SCRATCH, 3))
 		return NULL;
 	Py_BEGIN_ALLOW_THREADS
 	library.gated_feed_forward_backward(a.context, a.t[0], a.t[1], a.t[2], a.t[3], a.t[4], (float) a.number[0], a.t[5], (float) a.number[1], a.t[6], a.t[7], (int) a.number[2], a.t[8]);
@@ -178,7 +197,7 @@ static PyObject* gated_feed_forward_backward(PyObject *self, PyObject *const *ar
 static PyObject* softmax_cross_entropy_forward(PyObject *self, PyObject *const *args, Py_ssize_t given)
 {
 	Arguments a;
-	if (!take(&a, args, given, 6, 0))
+	if (!take(&a, args, given, 6, SCRATCH, 0))
 		return NULL;
 	Py_BEGIN_ALLOW_THREADS
 	library.softmax_cross_entropy_forward(a.context, a.t[0], a.t[1], a.t[2], a.t[3], a.t[4], a.t[5]);
@@ -188,7 +207,7 @@ static PyObject* softmax_cross_entropy_forward(PyObject *self, PyObject *const *
 static PyObject* softmax_cross_entropy_backward(PyObject *self, PyObject *const *args, Py_ssize_t given)
 {
 	Arguments a;
-	if (!take(&a, args, given, 8, 3))
+	if (!take(&a, args, given, 8, SCRATCH, 3))
 		return NULL;
 	Py_BEGIN_ALLOW_THREADS
 	library.softmax_cross_entropy_backward(a.context, a.t[0], a.t[1], a.t[2], a.t[3], (float) a.number[0], a.t[4], (float) a.number[1], a.t[5], (float) a.number[2], a.t[6], a.t[7]);
