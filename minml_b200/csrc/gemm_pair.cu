@@ -13,9 +13,11 @@
  * K and row tails are zero-filled by TMA, results are clipped by their tensor maps.
  *
  * The tensor core cuts its fp32 sums where an fp32 addition would round: measured, 1.6e-8 of the sum for every 16 K indices, always toward
- * zero (4.2e-6 at K = 4096).  That is nothing against a result rounded to fp16, but a loss is kept in fp32, and where a row is certain P - 1 is
- * the difference of two numbers near 1.  So both epilogues of logits add up accumulators of 1024 K indices each in registers, in the same order:
- * the gradient's logits are those that lse was made from, bit for bit.
+ * zero (4.2e-6 at K = 4096); where all terms have one sign 1e-7 (2.7e-5 at K = 4096, 1.7e-3 at 262 144).  A loss is kept in fp32, and where a
+ * row is certain P - 1 is the difference of two numbers near 1, so both epilogues of logits add up accumulators of 1024 K indices each in
+ * registers, in the same order: the gradient's logits are those that lse was made from, bit for bit.  Products that leave a plain result, among
+ * them all weight gradients, whose K is the number of tokens, add up accumulators of 8192 (5.3e-5, a ninth of the rounding to fp16).  Only the
+ * gated products, whose K is embed, take one accumulator for all of it.
  */
 #include "common.cuh"
 #include "tc.cuh"
@@ -46,7 +48,7 @@ namespace mb200
 		// of the 168 registers a thread starts with, what the first four warps give up is what the epilogue gets: 128 * 40 + 256 * 232 = 384 * 168
 		constexpr int REGISTERS_FEW = 40, REGISTERS_MANY = 232;
 		constexpr int HALF_BOX = 32 * 64, FLOAT_BOX = 32 * 128;
-		constexpr int LOGITS_SEGMENT = 1024 / BK; // K blocks per accumulator of a logit
+		constexpr int LOGITS_SEGMENT = 1024 / BK, RESULTS_SEGMENT = 8192 / BK; // K blocks per accumulator of a logit, and of a result rounded to fp16
 		constexpr int ROW_GROUP = 8; // tiles of 256 rows that neighbouring clusters share their columns over
 
 		enum Epilogue
@@ -67,7 +69,9 @@ namespace mb200
 				// per epilogue warp: four 32 x 32 boxes of fp16 or two of fp32; GATED_RECOMPUTE: all six boxes of a tile
 				static constexpr int staging_bytes = EPI == GATED_RECOMPUTE ? 6 * 2048 : 8192;
 				static constexpr int stages = EPI == GATED_RECOMPUTE ? 4 : 5;
-				static constexpr bool sums_segments = EPI == STATISTICS || EPI == PROBABILITIES; // the same logits, to the bit
+				// K blocks per accumulator; the two epilogues of logits have the same one and so the same logits, to the bit
+				static constexpr int segment = EPI == STATISTICS || EPI == PROBABILITIES ? LOGITS_SEGMENT : EPI == STORE || EPI == SUMS ? RESULTS_SEGMENT : 1 << 30;
+				static constexpr bool sums_segments = segment < 1 << 30;
 				static constexpr bool moves_registers = EPI == GATED || EPI == GATED_RECOMPUTE || sums_segments; // they hold 128 accumulators a thread
 				static constexpr int smem_bytes = stages * STAGE_BYTES + EPI_WARPS * staging_bytes + 1024;
 				static_assert(stages <= MAX_STAGES && smem_bytes <= 227 * 1024, "the configuration exceeds the SM");
@@ -187,7 +191,7 @@ namespace mb200
 				u.kb1 = min(k_blocks, u.kb0 + p.blocks_per_split);
 				return u;
 			};
-			constexpr int SEGMENT = Shape<EPI>::sums_segments ? LOGITS_SEGMENT : 1 << 30;
+			constexpr int SEGMENT = Shape<EPI>::segment;
 
 			if (threadIdx.x == 0)
 			{
@@ -494,15 +498,100 @@ namespace mb200
 						continue;
 					}
 
-					float scale = 1.0f;
-					bool active = true; // read under the multiplications
-					if (EPI == STORE)
+					if constexpr (EPI == SUMS || EPI == STORE)
 					{
-						scale = p.result.alpha * (p.result.alpha_device != nullptr ? *p.result.alpha_device : 1.0f);
-						if (p.result.row_scale != nullptr)
-							scale *= row_ok ? p.result.row_scale[row] : 0.0f;
-						active = p.result.row_scale == nullptr || (row_ok && p.result.row_scale[row] != 0.0f);
+						float scale = 1.0f;
+						bool active = true; // read under the multiplications
+						if (EPI == STORE)
+						{
+							scale = p.result.alpha * (p.result.alpha_device != nullptr ? *p.result.alpha_device : 1.0f);
+							if (p.result.row_scale != nullptr)
+								scale *= row_ok ? p.result.row_scale[row] : 0.0f;
+							active = p.result.row_scale == nullptr || (row_ok && p.result.row_scale[row] != 0.0f);
+						}
+						float all[BN / 2];
+						ok = sum_segments(u, all);
+						if (!ok)
+							break;
+#pragma unroll
+						for (int c = 0; c < BN / 64; c++)
+						{
+							const int n = u.nt * BN + half * (BN / 2) + c * 32;
+							if (n >= p.N)
+								break;
+							if (EPI == SUMS)
+							{
+								if (lane == 0)
+									bulk_wait_group_read<1>();
+								__syncwarp();
+								const uint32_t box = staging + (boxes++ % 2) * FLOAT_BOX;
+								uint32_t raw[32];
+#pragma unroll
+								for (int j = 0; j < 32; j++)
+									raw[j] = __float_as_uint(all[c * 32 + j]);
+								write_float_box(box, lane, raw);
+								publish();
+								if (lane == 0 && row0 < p.M)
+								{
+									if (p.accumulate)
+										tma_reduce_add_3d(&map_d, box, n, row0, u.split);
+									else
+										tma_store_3d(&map_d, box, n, row0, u.split);
+									bulk_commit_group();
+								}
+								continue;
+							}
+							float v[32];
+#pragma unroll
+							for (int j = 0; j < 32; j++)
+								v[j] = active ? all[c * 32 + j] * scale : 0.0f;
+							__half *dst = p.result.d + static_cast<long long>(row) * p.result.ldd + n;
+							if (p.result.beta != 0.0f && row_ok)
+							{
+								if (!p.direct && n + 32 <= p.N)
+								{
+#pragma unroll
+									for (int k = 0; k < 4; k++)
+										add_half8(v + 8 * k, reinterpret_cast<const uint4*>(dst)[k], p.result.beta);
+								}
+								else
+								{
+#pragma unroll
+									for (int j = 0; j < 32; j++)
+										if (n + j < p.N)
+											v[j] += p.result.beta * __half2float(dst[j]);
+								}
+							}
+							if (p.direct)
+							{ // rows that TMA cannot address: through a box, so that a store instruction covers 64 bytes of one row instead of 2 bytes of 32
+								write_half_box(staging, lane, v);
+								__syncwarp();
+								const int rows = min(32, p.M - row0);
+								if (n + lane < p.N)
+									for (int r = 0; r < rows; r++)
+									{
+										uint16_t bits;
+										asm volatile("ld.shared.u16 %0, [%1];" : "=h"(bits) : "r"(staging + r * 64 + (((lane / 8) ^ ((r >> 1) & 3)) * 16) + lane % 8 * 2) : "memory");
+										*reinterpret_cast<uint16_t*>(p.result.d + static_cast<long long>(row0 + r) * p.result.ldd + n + lane) = bits;
+									}
+								__syncwarp();
+								continue;
+							}
+							if (lane == 0)
+								bulk_wait_group_read<3>();
+							__syncwarp();
+							const uint32_t box = staging + (boxes++ % 4) * HALF_BOX;
+							write_half_box(box, lane, v);
+							publish();
+							if (lane == 0 && row0 < p.M)
+							{
+								tma_store_2d(&map_d, box, n, row0);
+								bulk_commit_group();
+							}
+						}
+						continue;
 					}
+
 					if (!wait_full())
 						break;
 					const uint32_t taddr = lane_base + (buffers & 1u) * BN;
@@ -636,14 +725,13 @@ namespace mb200
 						continue;
 					}
 
-#pragma unroll 1
-					for (int c = 0; c < BN / 64; c++)
+					if constexpr (EPI == GATED_BACKWARD)
 					{
-						const int n = u.nt * BN + half * (BN / 2) + c * 32;
-						float v[32];
-						if (EPI == GATED_BACKWARD)
+#pragma unroll 1
+						for (int c = 0; c < BN / 64; c++)
 						{
-							float a[32], b[32];
+							const int n = u.nt * BN + half * (BN / 2) + c * 32;
+							float v[32], a[32], b[32];
 							const int rows = min(32, p.M - row0);
 							const float *src = kept_block(p.kept, p, row0, n) + lane * 4;
 #pragma unroll
@@ -685,84 +773,6 @@ namespace mb200
 								tma_store_2d(&map_f, staging + 2 * HALF_BOX, n, row0);
 								bulk_commit_group();
 							}
-							continue;
-						}
-
-						load_chunk(taddr + half * (BN / 2) + c * 32, v);
-						if (c == BN / 64 - 1)
-							release();
-						if (n >= p.N)
-							continue;
-						if (EPI == SUMS)
-						{
-							if (lane == 0)
-								bulk_wait_group_read<1>();
-							__syncwarp();
-							const uint32_t box = staging + (boxes++ % 2) * FLOAT_BOX;
-							uint32_t raw[32];
-#pragma unroll
-							for (int j = 0; j < 32; j++)
-								raw[j] = __float_as_uint(v[j]);
-							write_float_box(box, lane, raw);
-							publish();
-							if (lane == 0 && row0 < p.M)
-							{
-								if (p.accumulate)
-									tma_reduce_add_3d(&map_d, box, n, row0, u.split);
-								else
-									tma_store_3d(&map_d, box, n, row0, u.split);
-								bulk_commit_group();
-							}
-							continue;
-						}
-						if (EPI == STORE)
-						{
-#pragma unroll
-							for (int j = 0; j < 32; j++)
-								v[j] = active ? v[j] * scale : 0.0f;
-							__half *dst = p.result.d + static_cast<long long>(row) * p.result.ldd + n;
-							if (p.result.beta != 0.0f && row_ok)
-							{
-								if (!p.direct && n + 32 <= p.N)
-								{
-#pragma unroll
-									for (int k = 0; k < 4; k++)
-										add_half8(v + 8 * k, reinterpret_cast<const uint4*>(dst)[k], p.result.beta);
-								}
-								else
-								{
-#pragma unroll
-									for (int j = 0; j < 32; j++)
-										if (n + j < p.N)
-											v[j] += p.result.beta * __half2float(dst[j]);
-								}
-							}
-							if (p.direct)
-							{ // rows that TMA cannot address: through a box, so that a store instruction covers 64 bytes of one row instead of 2 bytes of 32
-								write_half_box(staging, lane, v);
-								__syncwarp();
-								const int rows = min(32, p.M - row0);
-								if (n + lane < p.N)
-									for (int r = 0; r < rows; r++)
-									{
-										uint16_t bits;
-										asm volatile("ld.shared.u16 %0, [%1];" : "=h"(bits) : "r"(staging + r * 64 + (((lane / 8) ^ ((r >> 1) & 3)) * 16) + lane % 8 * 2) : "memory");
-										*reinterpret_cast<uint16_t*>(p.result.d + static_cast<long long>(row0 + r) * p.result.ldd + n + lane) = bits;
-									}
-								__syncwarp();
-								continue;
-							}
-						}
-						if (lane == 0)
-							bulk_wait_group_read<3>();
-						__syncwarp();
-						const uint32_t box = staging + (boxes++ % 4) * HALF_BOX;
-						write_half_box(box, lane, v);
-						publish();
-						if (lane == 0 && row0 < p.M)
-						{
-							tma_store_2d(&map_d, box, n, row0);
-							bulk_commit_group();
 						}
 					}
 				}
