@@ -10,7 +10,8 @@
  * 50 cycles each however few rows are real): then a cluster of 2, 4 or 8 CTAs takes each set of rows, one K range a CTA, and adds the
  * sums up through distributed shared memory in a fixed order.
  *   warp 0 TMA, warp 1 multiplications, warps 2-5 epilogue: a lane is a weight row, so results leave as 64 contiguous bytes a token.
- * Row statistics take an accumulator for every 1024 K indices and add them in fp32, because the tensor core cuts its sums (gemm_pair.cu).
+ * Row statistics take an accumulator for every 1024 K indices and add them in fp32, because the tensor core cuts its sums (gemm_pair.cu); those of
+ * a tile that do not fit a buffer of tensor memory (embed above 4096 for 64 tokens) come in several.
  * Measured, gated block of 4096 x 11008: 1 token 49 us (two launches, 270 MB: 5.5 TB/s), 64 tokens 61 us.  Above 64 rows the paired kernel
  * (gemm_pair.cu) is as fast or faster: 2048 x 8192, 128 rows 48 us here, 129 rows 39 us there.
  */
@@ -57,7 +58,7 @@ namespace mb200
 				int cluster; // CTAs that share a set of rows
 				int tiles, tile_groups; // tiles of every set, and the most groups one has
 				int blocks_per_stage, stages, block_bytes; // a stage: blocks_per_stage x (planes x tile_groups boxes, then the tokens' rows)
-				int segment_blocks;
+				int segment_blocks, pass_segments; // K blocks of an accumulator, accumulators that a buffer holds (STATISTICS)
 				int tmem_columns; // two buffers
 				__half *out;
 				int ldo;
@@ -236,16 +237,15 @@ namespace mb200
 				{
 					const uint32_t idesc = make_idesc_f16(p.columns);
 					int s = 0;
-					uint32_t parity = 0u;
+					uint32_t parity = 0u, buffers = 0;
 					bool ok = true;
-					for (int tile = 0; tile < tiles && ok; tile++)
+					for (int tile = 0; tile < tiles && ok; tile++, buffers++)
 					{
-						const uint32_t buffer = tile & 1u;
-						if (!mbar_wait(smem_u32(&bars.tmem_empty[buffer]), ((tile >> 1) & 1u) ^ 1u, abort_flag))
+						if (!mbar_wait(smem_u32(&bars.tmem_empty[buffers & 1u]), ((buffers >> 1) & 1u) ^ 1u, abort_flag))
 							break;
 						tcgen05_fence_after();
-						uint32_t d = tmem_base + buffer * (p.tmem_columns / 2);
-						int in_segment = 0;
+						uint32_t d = tmem_base + (buffers & 1u) * (p.tmem_columns / 2);
+						int in_segment = 0, segments = 0;
 						for (int kb = kb0; kb < kb1; kb += p.blocks_per_stage)
 						{
 							if (!mbar_wait(smem_u32(&bars.full[s]), parity, abort_flag))
@@ -258,6 +258,22 @@ namespace mb200
 							uint32_t base = smem_base + s * stage_bytes;
 							for (int j = 0; j < blocks; j++, base += p.block_bytes)
 							{
+								if (KIND == STATISTICS && in_segment == p.segment_blocks)
+								{ // the next accumulator, in the other buffer when this one is full
+									in_segment = 0;
+									d += p.columns;
+									if (++segments == p.pass_segments)
+									{
+										mma_commit(smem_u32(&bars.tmem_full[buffers & 1u]));
+										buffers++;
+										ok = mbar_wait(smem_u32(&bars.tmem_empty[buffers & 1u]), ((buffers >> 1) & 1u) ^ 1u, abort_flag);
+										if (!ok)
+											break;
+										tcgen05_fence_after();
+										d = tmem_base + (buffers & 1u) * (p.tmem_columns / 2);
+										segments = 0;
+									}
+								}
 								const uint64_t desc_x = make_desc_k_sw128(base + PLANES * plane_bytes);
 								const uint32_t accumulate = in_segment > 0 ? 1u : 0u;
 #pragma unroll
@@ -268,12 +284,10 @@ namespace mb200
 									for (int k = 0; k < 4; k++)
 										mma_ss<0>(d + plane * p.columns, desc_w + 2 * k, desc_x + 2 * k, idesc, accumulate | (k > 0 ? 1u : 0u));
 								}
-								if (++in_segment == p.segment_blocks)
-								{ // the next segment's accumulator
-									in_segment = 0;
-									d += p.columns;
-								}
+								in_segment++;
 							}
+							if (!ok)
+								break;
 							mma_commit(smem_u32(&bars.empty[s]));
 							if (++s == p.stages)
 							{
@@ -282,7 +296,7 @@ namespace mb200
 							}
 						}
 						if (ok)
-							mma_commit(smem_u32(&bars.tmem_full[buffer]));
+							mma_commit(smem_u32(&bars.tmem_full[buffers & 1u]));
 					}
 				}
 				__syncwarp();
@@ -290,58 +304,67 @@ namespace mb200
 			else
 			{ /* ------------------------------------------------------------ epilogue */
 				const int q = warp % 4;
-				const int segments = (kb1 - kb0 + p.segment_blocks - 1) / p.segment_blocks;
+				uint32_t buffers = 0;
+				auto wait_full = [&]() -> bool
+				{
+					if (!mbar_wait_warp(smem_u32(&bars.tmem_full[buffers & 1u]), (buffers >> 1) & 1u, abort_flag, 20u))
+						return false;
+					tcgen05_fence_after();
+					return true;
+				};
+				auto release = [&]()
+				{ // every load from this accumulator buffer has returned
+					tcgen05_fence_before();
+					__syncwarp();
+					if (lane == 0)
+						mbar_arrive(smem_u32(&bars.tmem_empty[buffers & 1u]));
+					buffers++;
+				};
 				for (int tile = 0; tile < tiles; tile++)
 				{
-					const uint32_t buffer = tile & 1u;
-					if (!mbar_wait_warp(smem_u32(&bars.tmem_full[buffer]), (tile >> 1) & 1u, abort_flag, 20u))
-						break;
-					tcgen05_fence_after();
 					const int n = first_group(tile) * GROUP + q * 32 + lane; // this lane's result column
 					const bool valid = q * 32 + lane < (first_group(tile + 1) - first_group(tile)) * GROUP && n < p.N;
-					const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + buffer * (p.tmem_columns / 2);
-					for (int c = 0; c < p.columns; c += 16)
+					const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
+					if constexpr (KIND == STATISTICS)
 					{
-						uint32_t r[16], r2[16];
-						tmem_ld_32x16(taddr + c, r);
-						if (KIND == GATED)
-							tmem_ld_32x16(taddr + p.columns + c, r2);
-						tmem_wait_ld();
-						float v[16];
-#pragma unroll
-						for (int j = 0; j < 16; j++)
-							v[j] = __uint_as_float(r[j]);
-						if (KIND == STATISTICS)
-							for (int s = 1; s < segments; s++)
-							{
-								tmem_ld_32x16(taddr + s * p.columns + c, r2);
-								tmem_wait_ld();
-#pragma unroll
-								for (int j = 0; j < 16; j++)
-									v[j] += __uint_as_float(r2[j]);
-							}
-						if (p.cluster > 1)
-						{ // this CTA's sums of [plane][token][row], over the ring: every stage has been read when the accumulators are full
-#pragma unroll
-							for (int j = 0; j < 16; j++)
-								if (c + j < p.tokens)
-								{
-									st_shared_f32(smem_base + ((c + j) * 128 + q * 32 + lane) * 4, v[j]);
-									if (KIND == GATED)
-										st_shared_f32(smem_base + ((p.tokens + c + j) * 128 + q * 32 + lane) * 4, __uint_as_float(r2[j]));
-								}
-							continue;
-						}
-						if (KIND == STATISTICS)
+						float z[FEW_TOKENS]; // this lane's column for every token, added up in fp32
+						bool ok = true;
+						for (int left = (kb1 - kb0 + p.segment_blocks - 1) / p.segment_blocks; left > 0; left -= p.pass_segments)
 						{
-							float sum[16];
+							const bool first = left + p.pass_segments > (kb1 - kb0 + p.segment_blocks - 1) / p.segment_blocks;
+							ok = wait_full();
+							if (!ok)
+								break;
+							const uint32_t taddr = lane_base + (buffers & 1u) * (p.tmem_columns / 2);
+#pragma unroll
+							for (int c = 0; c < FEW_TOKENS; c += 16)
+								if (c < p.columns)
+									for (int s = 0; s < min(left, p.pass_segments); s++)
+									{
+										uint32_t r[16];
+										tmem_ld_32x16(taddr + s * p.columns + c, r);
+										tmem_wait_ld();
+#pragma unroll
+										for (int j = 0; j < 16; j++)
+											z[c + j] = (first && s == 0 ? 0.0f : z[c + j]) + __uint_as_float(r[j]);
+									}
+							release();
+						}
+						if (!ok)
+							break;
+#pragma unroll
+						for (int c = 0; c < FEW_TOKENS; c += 16)
+						{
+							if (c >= p.columns)
+								break;
+							float v[16], sum[16];
 #pragma unroll
 							for (int j = 0; j < 16; j++)
 							{ // exponentials against the warp's maximum for the token
-								const float z = valid ? v[j] : -INFINITY, top = warp_max(z);
-								sum[j] = !valid || z == -INFINITY ? 0.0f : exp2_approx((z - top) * LOG2E);
+								const float mine = valid ? z[c + j] : -INFINITY, top = warp_max(mine);
+								sum[j] = !valid || mine == -INFINITY ? 0.0f : exp2_approx((mine - top) * LOG2E);
 								if (valid && c + j < p.tokens && p.targets[c + j] == n)
-									p.target_logit[c + j] = z;
+									p.target_logit[c + j] = mine;
 								v[j] = top;
 							}
 							// lane l ends with the sum (and takes the maximum) of token c + l % 16: each step halves the tokens a lane holds
@@ -360,6 +383,33 @@ namespace mb200
 							sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], 16);
 							if (lane < 16 && c + lane < p.tokens)
 								running[q][c + lane] = join(running[q][c + lane], make_float2(v[0], sum[0]));
+						}
+						continue;
+					}
+					if (!wait_full())
+						break;
+					const uint32_t taddr = lane_base + (buffers & 1u) * (p.tmem_columns / 2);
+					for (int c = 0; c < p.columns; c += 16)
+					{
+						uint32_t r[16], r2[16];
+						tmem_ld_32x16(taddr + c, r);
+						if (KIND == GATED)
+							tmem_ld_32x16(taddr + p.columns + c, r2);
+						tmem_wait_ld();
+						float v[16];
+#pragma unroll
+						for (int j = 0; j < 16; j++)
+							v[j] = __uint_as_float(r[j]);
+						if (p.cluster > 1)
+						{ // this CTA's sums of [plane][token][row], over the ring: every stage has been read when the accumulators are full
+#pragma unroll
+							for (int j = 0; j < 16; j++)
+								if (c + j < p.tokens)
+								{
+									st_shared_f32(smem_base + ((c + j) * 128 + q * 32 + lane) * 4, v[j]);
+									if (KIND == GATED)
+										st_shared_f32(smem_base + ((p.tokens + c + j) * 128 + q * 32 + lane) * 4, __uint_as_float(r2[j]));
+								}
 							continue;
 						}
 						if (!valid)
@@ -377,10 +427,7 @@ namespace mb200
 								*dst = __float2half_rn(p.beta != 0.0f ? v[j] + p.beta * __half2float(*dst) : v[j]);
 						}
 					}
-					tcgen05_fence_before();
-					__syncwarp();
-					if (lane == 0)
-						mbar_arrive(smem_u32(&bars.tmem_empty[buffer]));
+					release();
 				}
 			}
 
@@ -525,12 +572,11 @@ namespace mb200
 			p.segment_blocks = 1 << 30;
 			if (KIND == STATISTICS)
 			{
-				const int segments = std::min(BUFFER_COLUMNS / p.columns, (p.k_blocks + SEGMENT_BLOCKS - 1) / SEGMENT_BLOCKS);
+				const int segments = (p.k_blocks + SEGMENT_BLOCKS - 1) / SEGMENT_BLOCKS;
 				p.segment_blocks = (p.k_blocks + segments - 1) / segments;
+				p.pass_segments = std::min(segments, BUFFER_COLUMNS / p.columns);
 			}
-			int used = 2 * PLANES * p.columns;
-			if (KIND == STATISTICS)
-				used = 2 * p.columns * ((p.k_blocks + p.segment_blocks - 1) / p.segment_blocks);
+			const int used = 2 * p.columns * (KIND == STATISTICS ? p.pass_segments : PLANES);
 			for (p.tmem_columns = 32; p.tmem_columns < used;)
 				p.tmem_columns *= 2;
 			CUtensorMap map_w, map_w_less, map_x;
