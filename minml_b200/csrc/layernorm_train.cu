@@ -610,9 +610,10 @@ namespace mb200
 #pragma unroll
 					for (int j = 0; j < PAIRS; j++)
 					{
-						Pair v = pair_add(x[q].get(j), pair_of(-st[q].x)); // before the factor: a large mean must not cost the difference its digits
-						if (HAS_EXT)
+						Pair v = x[q].get(j);
+						if (HAS_EXT) // first, as in the forward pass: where x and ext cancel, their sum is exact and x - mean is not
 							v = pair_add(v, e[HAS_EXT ? q : 0].get(j));
+						v = pair_add(v, pair_of(-st[q].x)); // before the factor: a large mean must not cost the difference its digits
 						const Pair dv = d[q].get(j), gy = gamma != nullptr ? pair_mul(dv, g.get(j)) : dv;
 						xh[q][j] = pair_mul(v, pair_of(st[q].y));
 						t1 = pair_add(t1, gy);
@@ -811,9 +812,9 @@ namespace mb200
 					d.load(row + shape.row_bytes, lane, channels);
 #pragma unroll
 					for (int j = 0; j < PAIRS; j++)
-						xh[j] = pair_add(x.get(j), pair_of(-mean)); // before the factor: a large mean must not cost the difference its digits
+						xh[j] = x.get(j);
 					if (ext != nullptr)
-					{
+					{ // first, as in the forward pass: where x and ext cancel, their sum is exact and x - mean is not
 						x.load(row + 2 * shape.row_bytes, lane, channels);
 #pragma unroll
 						for (int j = 0; j < PAIRS; j++)
@@ -823,7 +824,8 @@ namespace mb200
 					for (int j = 0; j < PAIRS; j++)
 					{
 						const Pair dv = d.get(j), gy = gamma != nullptr ? pair_mul(dv, g.get(j)) : dv;
-						xh[j] = pair_mul(xh[j], pair_of(inv_stddev));
+						// the mean before the factor: a large one must not cost the difference its digits
+						xh[j] = pair_mul(pair_add(xh[j], pair_of(-mean)), pair_of(inv_stddev));
 						t1 = pair_add(t1, gy);
 						t2 = pair_fma(gy, xh[j], t2);
 						sum_w[j] = pair_fma(dv, xh[j], sum_w[j]);
