@@ -374,12 +374,51 @@ def _refuse(t, device_index):
     raise BackendError("a dense row-major tensor of at most 6 dimensions is needed, not %s with strides %s" % (tuple(t.shape), t.stride()))
 
 
+class CtypesCalls:
+    """What the extension module does (csrc/binding.c), through ctypes, for where it cannot be built: no C compiler, no Python headers, another interpreter
+    than the one it was built for.  A layer norm's two calls take the host 10 us longer."""
+    # C arguments behind the context: t a tensor, n a number, i an integer, w scratch memory
+    _FORMS = {"layernorm_forward": "tttttt", "layernorm_backward": "tttttntnttw", "gated_feed_forward_forward": "tttntitw", "gated_feed_forward_backward": "tttttntnttiw",
+              "softmax_cross_entropy_forward": "tttttw", "softmax_cross_entropy_backward": "ttttntntntw"}
+
+    def __getattr__(self, name):
+        form, function = self._FORMS[name], getattr(lib, "mb200_" + name)
+        tensors = [c for c in form if c in "tw"]
+
+        def call(handle, device_index, *given):
+            if len(given) != len(form):
+                raise TypeError("%d arguments expected, %d given" % (2 + len(form), 2 + len(given)))
+            described = iter([self._describe(t, device_index, c == "w") for t, c in zip(given, tensors)])
+            numbers = iter(given[len(tensors):])
+            function(handle, *[next(described) if c in "tw" else int(next(numbers)) if c == "i" else ctypes.c_float(next(numbers)) for c in form])
+            message = _last_error(handle)
+            if message:
+                lib.mb200_clear_last_error(handle)
+                raise BackendError(message)
+        setattr(self, name, call)
+        return call
+
+    @staticmethod
+    def _describe(t, device_index, scratch):
+        if t is None:
+            return _EMPTY
+        if t.get_device() != device_index or not t.is_contiguous() or t.dim() > 6:
+            _refuse(t, device_index)
+        shape = t.shape
+        if any(n > 0x7FFFFFFF for n in shape):
+            if not scratch or t.numel() // 256 > 0x7FFFFFFF:
+                _refuse(t, device_index)
+            shape = (t.numel() // 256, 256)  # its shape says nothing but its size
+        rank = len(shape)
+        return mlTensor_t.from_buffer_copy(_PACK(t.data_ptr(), _DTYPES.get(t.dtype, _abi.DTYPE_UNKNOWN), rank, *shape, *_FILL[rank]))
+
+
 def _load_binding():
     """The functions below describe up to nine tensors a call, which an extension module does in a fraction of the time (csrc/binding.c)."""
     try:
         from . import _binding
-    except ImportError as e:
-        raise RuntimeError("minml_b200/_binding.so is missing or does not load (%s): run `python -m minml_b200.build`" % e)
+    except ImportError:
+        return CtypesCalls()
     names = [name for name in _abi.declared_symbols() if name.startswith("mb200_")]
     _binding.bind({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in names}, _DTYPES, _refuse, BackendError)
     return _binding

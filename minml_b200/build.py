@@ -3,8 +3,9 @@
 Usage:  python -m minml_b200.build [--force] [--verbose]
 
 Each .cu file under minml_b200/csrc is compiled to an object file (in parallel) and the objects are linked into
-minml_b200/libminml_b200.so, and csrc/binding.c to the extension module minml_b200/_binding.so.  Objects are rebuilt only when their source or a header is newer.  The library links
-the CUDA runtime statically and fetches the one driver entry point it needs (cuTensorMapEncodeTiled) at run time,
+minml_b200/libminml_b200.so, and csrc/binding.c to the extension module minml_b200/_binding.*.so of the running interpreter (without a C compiler or
+Python's headers there is none, and backend.py calls the library through ctypes).  Objects are rebuilt only when their source or a header is newer.  The
+library links the CUDA runtime statically and fetches the one driver entry point it needs (cuTensorMapEncodeTiled) at run time,
 so it has no link-time dependency on libcuda.
 """
 import os
@@ -18,7 +19,7 @@ ROOT = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(ROOT, "csrc")
 OBJ = os.path.join(ROOT, "build")
 LIB = os.path.join(ROOT, "libminml_b200.so")
-BINDING = os.path.join(ROOT, "_binding.so")
+BINDING = os.path.join(ROOT, "_binding" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 HEADER = os.path.join(ROOT, "..", "include", "minml_b200.h")
 
 NVCC_FLAGS = [
@@ -45,9 +46,15 @@ def build_binding(force=False):
     source = os.path.join(CSRC, "binding.c")
     if force or not os.path.exists(BINDING) or os.path.getmtime(BINDING) < max(os.path.getmtime(source), os.path.getmtime(HEADER)):
         cmd = [os.environ.get("CC") or "gcc", "-O2", "-Wall", "-shared", "-fPIC", "-I", sysconfig.get_paths()["include"], "-I", os.path.dirname(HEADER), "-o", BINDING, source]
-        proc = subprocess.run(cmd, capture_output=True, text=True)
+        try:
+            proc = subprocess.run(cmd, capture_output=True, text=True)
+        except OSError as e:
+            raise RuntimeError("building the extension module failed: %s" % e)
         if proc.returncode != 0:
             raise RuntimeError("building the extension module failed:\n%s\n%s" % (proc.stdout, proc.stderr))
+        untagged = os.path.join(ROOT, "_binding.so")  # of builds whose module any interpreter would have tried to load
+        if BINDING != untagged and os.path.exists(untagged):
+            os.remove(untagged)
     return BINDING
 
 
@@ -86,7 +93,10 @@ def build(force=False, verbose=False):
         proc = subprocess.run(cmd, capture_output=True, text=True)
         if proc.returncode != 0:
             raise RuntimeError("link failed:\n%s\n%s" % (proc.stdout, proc.stderr))
-    build_binding(force)
+    try:
+        build_binding(force)
+    except RuntimeError as e:  # the library is complete without it
+        print("%s\nThe backend will call the library through ctypes." % e, file=sys.stderr)
     return LIB
 
 
