@@ -19,7 +19,7 @@ namespace mb200
 	}
 	/* 1 / (1 + 2^(-g log2 e)) of two values with one reciprocal, 1 / a = b / (a b): the special-function unit is what an epilogue with this gate
 	 * runs out of first (three instead of four of its instructions for two values).  The power is held at 2^60 so that the product stays
-	 * finite: a sigmoid below 2^-60 comes out as 2^-60, which fp16 rounds to the same 0. */
+	 * finite, and a sigmoid that would be less than 2^-60 is 0 (2^-60 is not: g and u of 4e5 make 0.1 of it).  A NaN comes out as 2^-60. */
 	__device__ __forceinline__ Pair sigmoid_fast(Pair g)
 	{
 		const Pair t = pair_mul(g, Pair { -1.44269504f, -1.44269504f });
@@ -28,7 +28,8 @@ namespace mb200
 		asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(fminf(t.y, 60.0f)));
 		e = pair_add(e, Pair { 1.0f, 1.0f });
 		const float r = reciprocal_approx(e.x * e.y);
-		return pair_mul(Pair { r, r }, Pair { e.y, e.x });
+		const Pair s = pair_mul(Pair { r, r }, Pair { e.y, e.x });
+		return Pair { t.x > 60.0f ? 0.0f : s.x, t.y > 60.0f ? 0.0f : s.y };
 	}
 	template<int GATE, bool FAST>
 	__device__ __forceinline__ void gate_with_derivative(float g, float &value, float &derivative)
