@@ -320,6 +320,10 @@ namespace mb200
 			return Plan(ctx, q, nullptr, training, std::min(MIN_PIECE, best)).bytes <= bytes ? std::min(MIN_PIECE, best) : 0;
 		}
 
+		bool fits_indices(const Problem &q)
+		{
+			return q.tokens <= MAX_EXTENT && q.vocab <= MAX_EXTENT && q.embed <= MAX_EXTENT;
+		}
 		bool check_problem(mlContext_t ctx, const char *who, const mlTensor_t &x, const mlTensor_t &w, const mlTensor_t &targets, Problem &q)
 		{
 			if (!check_extents(ctx, who, "x", x) || !check_extents(ctx, who, "weights", w))
@@ -338,9 +342,9 @@ namespace mb200
 			q.vocab = w.dim[0];
 			q.embed = w.dim[1];
 			q.tokens = volume(x) / q.embed;
-			if (q.tokens > 0x7FFFFFFFll)
+			if (!fits_indices(q))
 			{
-				record_error(ctx, "%s: %lld tokens are too many for one call", who, q.tokens);
+				record_error(ctx, "%s: %lld tokens, %d columns and an embed of %d are too many for one call", who, q.tokens, q.vocab, q.embed);
 				return false;
 			}
 			return check_operand(ctx, who, "x", x, x.dtype, q.tokens, q.embed) && check_operand(ctx, who, "weights", w, x.dtype, q.vocab, q.embed)
@@ -408,9 +412,9 @@ namespace mb200
 		}
 		void forward_float(mlContext_t ctx, const Problem &q, const Rows &rows, const Plan &plan, const Operands<float> &o, float *loss, float *lse)
 		{
-			for (int first = 0; first < q.vocab; first += plan.piece)
+			for (long long begin = 0; begin < q.vocab; begin += plan.piece)
 			{
-				const int width = std::min(plan.piece, q.vocab - first);
+				const int first = static_cast<int>(begin), width = std::min(plan.piece, q.vocab - first);
 				if (!float_product(ctx, static_cast<int>(q.tokens), width, q.embed, FloatOperand { o.x, plan.embed, false },
 						FloatOperand { o.w + static_cast<size_t>(first) * plan.embed, plan.embed, false }, plan.z, plan.pitch, 0.0f, plan.partials))
 					return;
@@ -443,9 +447,9 @@ namespace mb200
 					return;
 			}
 			const T *weighted_x = reinterpret_cast<const T*>(plan.weighted_x);
-			for (int first = 0; first < q.vocab; first += plan.piece)
+			for (long long begin = 0; begin < q.vocab; begin += plan.piece)
 			{
-				const int width = std::min(plan.piece, q.vocab - first);
+				const int first = static_cast<int>(begin), width = std::min(plan.piece, q.vocab - first);
 				const T *w = o.w + static_cast<size_t>(first) * ld;
 				if constexpr (half)
 				{
@@ -494,7 +498,7 @@ extern "C"
 		if (context == nullptr || x_shape.rank < 1 || x_shape.rank > 6 || w_shape.rank != 2 || w_shape.dim[0] <= 0 || w_shape.dim[1] <= 0 || last_dim(x_shape) != w_shape.dim[1])
 			return 0;
 		const Problem q { dtype, volume_without_last_dim(x_shape), w_shape.dim[1], w_shape.dim[0] };
-		if (q.tokens <= 0 || q.tokens > 0x7FFFFFFFll || (dtype != DTYPE_FLOAT16 && dtype != DTYPE_FLOAT32))
+		if (q.tokens <= 0 || !fits_indices(q) || (dtype != DTYPE_FLOAT16 && dtype != DTYPE_FLOAT32))
 			return 0;
 		// the forward call of a training step takes its scratch from the same workspace
 		const size_t forward = Plan(context, q, nullptr, false, recommended_piece(q, false)).bytes;

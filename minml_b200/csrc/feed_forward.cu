@@ -323,6 +323,10 @@ namespace mb200
 			return false;
 		}
 
+		bool fits_indices(const Problem &p)
+		{ // (of w1: two padded rows for every hidden unit)
+			return p.tokens <= MAX_EXTENT / 2 && p.hidden <= MAX_EXTENT / 2 && p.embed <= MAX_EXTENT;
+		}
 		bool check_problem(mlContext_t ctx, const char *who, const mlTensor_t &x, const mlTensor_t &w1, const mlTensor_t &w2, int gate, Problem &p)
 		{
 			if (!check_extents(ctx, who, "x", x) || !check_extents(ctx, who, "w1", w1) || !check_extents(ctx, who, "w2", w2))
@@ -347,9 +351,9 @@ namespace mb200
 			p.hidden = w1.dim[0] / 2;
 			p.gate = gate;
 			p.tokens = volume(x) / p.embed;
-			if (p.tokens > 0x3FFFFFFF)
+			if (!fits_indices(p))
 			{
-				record_error(ctx, "%s: %lld tokens are too many for one call", who, p.tokens);
+				record_error(ctx, "%s: %lld tokens, %d hidden units and an embed of %d are too many for one call", who, p.tokens, p.hidden, p.embed);
 				return false;
 			}
 			return check_operand(ctx, who, "x", x, x.dtype, p.tokens, p.embed) && check_operand(ctx, who, "w1", w1, x.dtype, 2ll * p.hidden, p.embed)
@@ -367,7 +371,7 @@ extern "C"
 		if (context == nullptr || x_shape.rank < 1 || x_shape.rank > 6 || w1_shape.rank != 2 || w1_shape.dim[0] <= 0 || w1_shape.dim[1] <= 0 || last_dim(x_shape) != w1_shape.dim[1])
 			return 0;
 		const Problem p { dtype, volume_without_last_dim(x_shape), w1_shape.dim[1], w1_shape.dim[0] / 2, MB200_GATE_SILU };
-		if (p.tokens <= 0 || p.tokens > 0x3FFFFFFF || (dtype != DTYPE_FLOAT16 && dtype != DTYPE_FLOAT32))
+		if (p.tokens <= 0 || !fits_indices(p) || (dtype != DTYPE_FLOAT16 && dtype != DTYPE_FLOAT32))
 			return 0;
 		return std::max(Plan(context, p, nullptr, false, training && saved, nullptr).bytes, training ? Plan(context, p, nullptr, true, saved, nullptr).bytes : 0);
 	}

@@ -1166,6 +1166,7 @@ extern "C"
 		MB200_REQUIRE(context, x.dtype == DTYPE_FLOAT16 || x.dtype == DTYPE_FLOAT32, "%s: x is %s, fp16 or fp32 expected", who, dtype_name(x.dtype));
 		const int channels = last_dim(x);
 		MB200_REQUIRE(context, channels >= 2, "%s: the unbiased variance needs at least 2 channels", who);
+		MB200_REQUIRE(context, channels <= MAX_EXTENT, "%s: rows of %d channels are too long", who, channels);
 		const long long rows = volume(x) / channels;
 		if (!check_operand(context, who, "x", x, x.dtype, rows, channels) || !check_operand(context, who, "y", y, x.dtype, rows, channels)
 				|| !check_operand(context, who, "stats", stats, DTYPE_FLOAT32, rows, 2)
@@ -1207,7 +1208,7 @@ extern "C"
 
 	size_t mb200_layernorm_backward_get_workspace_size(mlContext_t context, mlShape_t shape)
 	{
-		if (context == nullptr || shape.rank < 1 || shape.rank > 6 || last_dim(shape) < 2)
+		if (context == nullptr || shape.rank < 1 || shape.rank > 6 || last_dim(shape) < 2 || last_dim(shape) > MAX_EXTENT)
 			return 0;
 		const long long rows = volume_without_last_dim(shape);
 		return rows <= 0 ? 0 : static_cast<size_t>(2) * partial_rows(get(context)->sm_count, rows, last_dim(shape)) * last_dim(shape) * sizeof(float);
@@ -1222,6 +1223,7 @@ extern "C"
 		MB200_REQUIRE(context, x.dtype == DTYPE_FLOAT16 || x.dtype == DTYPE_FLOAT32, "%s: x is %s, fp16 or fp32 expected", who, dtype_name(x.dtype));
 		const int channels = last_dim(x);
 		MB200_REQUIRE(context, channels >= 2, "%s: the unbiased variance needs at least 2 channels", who);
+		MB200_REQUIRE(context, channels <= MAX_EXTENT, "%s: rows of %d channels are too long", who, channels);
 		const long long rows = volume(x) / channels;
 		const mlDataType_t grad = !is_empty_descriptor(dw) ? dw.dtype : !is_empty_descriptor(db) ? db.dtype : DTYPE_FLOAT32;
 		MB200_REQUIRE(context, grad == DTYPE_FLOAT32 || grad == x.dtype, "%s: the weight gradients are %s, fp32 or the type of x expected", who, dtype_name(grad));

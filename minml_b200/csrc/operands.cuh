@@ -32,7 +32,9 @@ namespace mb200
 				return "another type";
 		}
 	}
-	/* A rank within the descriptor's array and no negative extent: what every later use of dim[] relies on. */
+	/* Rows and columns of a matrix at most: the kernels' 32-bit indices pass the end by less than 4096 (a tile, the step of a loop). */
+	constexpr long long MAX_EXTENT = 0x7FFFF000;
+	/* A rank within the descriptor's array, no negative extent and a volume of 64 bits in bytes: what every later use of dim[] relies on. */
 	inline bool check_extents(mlContext_t ctx, const char *who, const char *name, const mlTensor_t &t)
 	{
 		if (t.rank < 1 || t.rank > 6)
@@ -46,6 +48,16 @@ namespace mb200
 				record_error(ctx, "%s: %s has a negative extent", who, name);
 				return false;
 			}
+		long long elements = 1;
+		for (int i = 0; i < t.rank && elements != 0; i++)
+		{
+			if (t.dim[i] > 0 && elements > (1ll << 59) / t.dim[i])
+			{
+				record_error(ctx, "%s: %s has more elements than any memory", who, name);
+				return false;
+			}
+			elements *= t.dim[i];
+		}
 		return true;
 	}
 	/* `t` holds rows x columns elements of `dtype`: a matrix whose leading extents multiply to `rows` and whose last is `columns`, or, for
