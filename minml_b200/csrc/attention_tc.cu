@@ -452,7 +452,6 @@ namespace mb200
 		p.status = c->dev_status;
 		kernel_mha_tc<<<dim3(heads, batch), NT, smem, stream>>>(map_q, map_k, p);
 		MB200_COUNT_LAUNCH();
-		c->kernels_with_waits = true;
 		return check_cuda(ctx, cudaGetLastError(), "cuda_multi_head_attention_forward (tcgen05)");
 	}
 } /* namespace mb200 */

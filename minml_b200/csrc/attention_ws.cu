@@ -746,7 +746,6 @@ namespace mb200
 		if (!launched)
 			return false;
 		MB200_COUNT_LAUNCH();
-		c->kernels_with_waits = true;
 #if MB200_MHA_TRACE
 		if (trace != nullptr)
 		{

@@ -60,8 +60,9 @@ namespace mb200
 			PendingInt8 pending_i8;
 			std::recursive_mutex mutex; // guards `pending`, `pending_i8` and `fusion` (recursive: a flush re-enters the eager entry points)
 			int sm_count = 148;
-			bool kernels_with_waits = false; // a kernel that polls mbarriers ran since the last synchronize
-			int *dev_status = nullptr; // device word set to non-zero by a kernel whose bounded wait ran out
+			// a word that a kernel whose bounded wait ran out sets to non-zero, also in a replayed graph: host memory, so that every synchronize can look
+			volatile int *status = nullptr;
+			int *dev_status = nullptr; // its address on the device
 	};
 
 	extern std::atomic<unsigned long long> g_launch_count;

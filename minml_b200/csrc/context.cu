@@ -275,8 +275,14 @@ extern "C"
 			delete c;
 			return nullptr;
 		}
-		if (check_cuda(nullptr, cudaMalloc(reinterpret_cast<void**>(&c->dev_status), sizeof(int)), "cuda_create_context: status word"))
-			cudaMemset(c->dev_status, 0, sizeof(int));
+		void *status = nullptr, *on_device = nullptr;
+		if (check_cuda(nullptr, cudaHostAlloc(&status, sizeof(int), cudaHostAllocMapped), "cuda_create_context: status word"))
+		{
+			c->status = reinterpret_cast<volatile int*>(status);
+			*c->status = 0;
+			if (check_cuda(nullptr, cudaHostGetDevicePointer(&on_device, status, 0), "cuda_create_context: status word"))
+				c->dev_status = reinterpret_cast<int*>(on_device);
+		}
 		std::lock_guard<std::mutex> lock(g_contexts_mutex);
 		g_contexts.push_back(c);
 		return c;
@@ -292,15 +298,10 @@ extern "C"
 		flush_pending(context);
 		check_cuda(context, cudaStreamSynchronize(use_stream(context)), "cuda_synchronize_with_context");
 		Context *c = get(context);
-		if (c->dev_status != nullptr && c->kernels_with_waits)
+		if (c->status != nullptr && *c->status != 0)
 		{
-			int status = 0;
-			if (check_cuda(context, cudaMemcpy(&status, c->dev_status, sizeof(int), cudaMemcpyDeviceToHost), "status word read") && status != 0)
-			{
-				record_error(context, "a tensor-core kernel gave up on a bounded wait (status %d); its output is incomplete", status);
-				cudaMemset(c->dev_status, 0, sizeof(int));
-			}
-			c->kernels_with_waits = false;
+			record_error(context, "a tensor-core kernel gave up on a bounded wait (status %d); its output is incomplete", *c->status);
+			*c->status = 0;
 		}
 	}
 	bool cuda_is_context_ready(mlContext_t context)
@@ -333,8 +334,8 @@ extern "C"
 		cudaStreamDestroy(c->stream);
 		if (c->workspace != nullptr)
 			cudaFree(c->workspace);
-		if (c->dev_status != nullptr)
-			cudaFree(c->dev_status);
+		if (c->status != nullptr)
+			cudaFreeHost(const_cast<int*>(c->status));
 		delete c;
 	}
 

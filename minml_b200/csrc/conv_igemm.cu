@@ -925,7 +925,6 @@ namespace mb200
 			const int grid = std::min(tiles, get(ctx)->sm_count);
 			kernel_conv3x3_igemm<KIND, BN, TMA_A, 1, MT> <<<grid, Roles<KIND, TMA_A>::threads, C::smem_bytes, use_stream(ctx)>>>(map_w, map_x, p);
 			MB200_COUNT_LAUNCH();
-			get(ctx)->kernels_with_waits = true;
 			return check_cuda(ctx, cudaGetLastError(), "conv_igemm launch");
 		}
 
@@ -972,7 +971,6 @@ namespace mb200
 			config.gridDim = dim3(2 * std::min(units, max_clusters[device]), 1, 1);
 			const cudaError_t status = cudaLaunchKernelEx(&config, kernel_conv3x3_igemm<KIND, BN, true, 2, 1>, map_w, map_x, p);
 			MB200_COUNT_LAUNCH();
-			get(ctx)->kernels_with_waits = true;
 			return check_cuda(ctx, status, "conv_igemm pair launch") && check_cuda(ctx, cudaGetLastError(), "conv_igemm pair launch");
 		}
 

@@ -435,7 +435,6 @@ namespace mb200
 		const int grid = std::min(units, c->sm_count);
 		kernel_conv3x3_slab<<<grid, THREADS, smem, use_stream(ctx)>>>(map_w, map_x, p);
 		MB200_COUNT_LAUNCH();
-		c->kernels_with_waits = true;
 		return check_cuda(ctx, cudaGetLastError(), "conv_slab launch");
 	}
 } /* namespace mb200 */

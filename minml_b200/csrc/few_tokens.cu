@@ -602,7 +602,6 @@ namespace mb200
 			config.numAttrs = 2;
 			const cudaError_t status = cudaLaunchKernelEx(&config, kernel_few_tokens<KIND, GATE>, map_w, map_w_less, map_x, p);
 			MB200_COUNT_LAUNCH();
-			c->kernels_with_waits = true;
 			return check_cuda(ctx, status, "few_tokens launch");
 		}
 	}

@@ -612,7 +612,6 @@ namespace mb200
 		config.numAttrs = 2;
 		const cudaError_t status = cudaLaunchKernelEx(&config, kernel_gemm_fp32, map_a, map_b, map_d, p);
 		MB200_COUNT_LAUNCH();
-		c->kernels_with_waits = true;
 		if (!check_cuda(ctx, status, "gemm_fp32 launch"))
 			return false;
 		return splits == 1 || finish_sums<float>(ctx, d, ldd, M, N, partials, p.ldd, splits, 1.0f, nullptr, nullptr, beta);

@@ -865,7 +865,6 @@ namespace mb200
 			config.numAttrs = 2;
 			const cudaError_t status = cudaLaunchKernelEx(&config, kernel_gemm_pair<EPI, GATE>, maps.a, maps.b, maps.d, maps.e, maps.f, maps.dy, maps.w2, p);
 			MB200_COUNT_LAUNCH();
-			c->kernels_with_waits = true;
 			return check_cuda(ctx, status, "gemm_pair launch");
 		}
 

@@ -994,7 +994,6 @@ namespace mb200
 		p.inv_out_scale = 1.0f / g.out_scale; // AffineTransform::get_inverse of the reference's host code
 		p.inv_out_shift = -g.out_shift / g.out_scale;
 		p.status = c->dev_status;
-		c->kernels_with_waits = true;
 
 		if (g.kind == 3)
 			return launch<3, 128>(ctx, stream, map_a, map_b, map_a, map_a, p, c->sm_count);

@@ -1052,7 +1052,6 @@ namespace mb200
 					record_error(ctx, "layer norm: %d bytes of shared memory are not available", RING_BYTES);
 					return;
 				}
-				get(ctx)->kernels_with_waits = true;
 				if (backward)
 					kernel_layernorm_backward_ring<T, W, E> <<<a.blocks, W, shape.stages * stage_bytes, stream>>>(a.out, a.x, a.ext, a.dy, a.gamma, a.stats, a.beta_dx, a.partial, a.rows,
 							a.channels, shape, a.status);

@@ -156,7 +156,6 @@ extern "C"
 		}
 		if (!launched)
 			return -1.0;
-		c->kernels_with_waits = true;
 		long long host[2] = { 0, 0 };
 		if (!check_cuda(context, cudaGetLastError(), "mb200_probe_mma_cycles launch")
 				|| !check_cuda(context, cudaMemcpyAsync(host, out, sizeof(host), cudaMemcpyDeviceToHost, stream), "mb200_probe_mma_cycles read")
@@ -173,7 +172,6 @@ extern "C"
 		Context *c = get(context);
 		kernel_wait_that_runs_out <<<1, 64, 0, use_stream(context)>>>(c->dev_status, static_cast<unsigned>(polls));
 		MB200_COUNT_LAUNCH();
-		c->kernels_with_waits = true;
 		check_cuda(context, cudaGetLastError(), "mb200_selftest_bounded_wait");
 	}
 }
