@@ -32,7 +32,7 @@ def dtype_of(t):
 
 
 def shape_of(t_or_dims):
-    dims = t_or_dims.shape if isinstance(t_or_dims, torch.Tensor) else t_or_dims
+    dims = t_or_dims.shape if isinstance(t_or_dims, torch.Tensor) else [int(d) for d in t_or_dims]
     rank = len(dims)
     return mlShape_t.from_buffer_copy(_PACK_SHAPE(rank, *dims, *_FILL[rank]))
 
@@ -45,16 +45,15 @@ def _check_device(t, ctx):
 
 
 _PACK_SHAPE = struct.Struct("@7i").pack  # the layout of mlShape_t
-_EMPTY = mlTensor_t()  # null data, rank 0 (passed by value, so one instance serves every absent operand)
-_EMPTY.dtype = _abi.DTYPE_UNKNOWN
 _PACK = struct.Struct("@Qii6i").pack  # the layout of mlTensor_t; packing at once costs half of setting the fields one by one
 _FILL = [(0,) * (6 - i) for i in range(7)]
+_EMPTY = _PACK(0, _abi.DTYPE_UNKNOWN, 0, *_FILL[0])
 
 
 def desc(t, ctx=None):
     """mlTensor_t for a dense torch tensor; None gives the empty descriptor (null data, rank 0)."""
     if t is None:
-        return _EMPTY
+        return mlTensor_t.from_buffer_copy(_EMPTY)
     assert t.is_contiguous(), "the backend ABI addresses dense row-major tensors only"
     if ctx is not None:
         _check_device(t, ctx)
@@ -401,7 +400,7 @@ class CtypesCalls:
     @staticmethod
     def _describe(t, device_index, scratch):
         if t is None:
-            return _EMPTY
+            return mlTensor_t.from_buffer_copy(_EMPTY)
         if t.get_device() != device_index or not t.is_contiguous() or t.dim() > 6:
             _refuse(t, device_index)
         shape = t.shape
