@@ -87,3 +87,27 @@ def test_log_sum_of_rows_over_a_long_embed(ctx, embed, tokens):
     want = torch.logsumexp(z, 1)
     assert float(want.min()) > 30 and float(z[:, 1:].max()) < 8
     assert float(((lse.double() - want).abs() / want).max()) <= 7.7e-6 + 16 * 2.0 ** -24 + 4 * 2.0 ** -23
+
+
+def test_fp32_products_over_a_long_sum(ctx):
+    """y = h W2^T with K = 8192 terms of one sign and h exact (the gate is 1, u picks elements of x, of 20 bits).  An accumulator takes 32 indices, 12
+    instructions with two cuts of 2^-23 each at most: 12 * 2^-22; the dropped product of the lower terms is at most 2^-20 and their rounding 2^-21:
+    4.4e-6 in all.  The 256 additions of fp32 round by half a step either way: in the mean over 2.4 million results nothing.  (74 tiles: one range of
+    K.)  One accumulator for all of K would come out 1 024 * 3 / 2 * 2^-22 = 3.7e-4 low at most; 5.7e-5 was measured."""
+    from minml_b200 import backend as B
+    tokens, embed, hidden = 512, 4736, 8192
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randint(2 ** 18, 3 * 2 ** 18, (tokens, embed), device="cuda", generator=gen).float() * 2.0 ** -19
+    x[:, 0] = 1.0
+    taken = torch.randint(0, embed, (hidden,), device="cuda", generator=gen)
+    w1 = torch.zeros((2 * hidden, embed), device="cuda")
+    w1[:hidden, 0] = 1.0
+    w1[hidden + torch.arange(hidden, device="cuda"), taken] = 1.0
+    w2 = torch.rand((embed, hidden), device="cuda", generator=gen) + 0.5
+    y = torch.empty_like(x)
+    ws = torch.empty(B.gatedFeedForwardGetWorkspaceSize(ctx, x.shape, w1.shape, x.dtype), device="cuda", dtype=torch.uint8)
+    B.gatedFeedForwardForward(ctx, x, w1, w2, y, "relu", workspace=ws)
+    ctx.synchronize()
+    off = y.double() / (x[:, taken].double() @ w2.double().T) - 1
+    assert abs(float(off.mean())) <= 4.4e-6, float(off.mean())
+    assert float(off.abs().max()) <= 4.4e-6 + 128 * 2.0 ** -24
