@@ -272,7 +272,7 @@ namespace mb200
 						if (tokens <= FEW_TOKENS && au == nullptr)
 						{ // decoding: both launches stream their weights once
 							if (few_gated(ctx, FewTokens { tokens, plan.embed, x, plan.embed, w1, plan.embed }, plan.hidden, p.gate, reinterpret_cast<__half*>(plan.h), plan.hidden))
-								few_product(ctx, FewTokens { tokens, plan.hidden, h, plan.hidden, w2, plan.hidden }, p.embed, y, p.embed, beta, true);
+								few_product_after_gated(ctx, FewTokens { tokens, plan.hidden, h, plan.hidden, w2, plan.hidden }, p.embed, y, p.embed, beta);
 							return;
 						}
 					if (gate(au))

@@ -63,7 +63,6 @@ namespace mb200
 				__half *out;
 				int ldo;
 				float beta;
-				int after_gated;
 				const int *targets;
 				float2 *parts;
 				int part_groups;
@@ -107,6 +106,7 @@ namespace mb200
 				const __grid_constant__ CUtensorMap map_w_less, const __grid_constant__ CUtensorMap map_x, const Params p)
 		{
 			constexpr int PLANES = KIND == GATED ? 2 : 1;
+			constexpr bool AFTER_GATED = KIND == PRODUCT;
 			extern __shared__ uint8_t smem_raw[];
 			__shared__ Barriers bars;
 			__shared__ float2 running[KIND == STATISTICS ? 4 : 1][KIND == STATISTICS ? FEW_TOKENS : 1];
@@ -153,7 +153,7 @@ namespace mb200
 			tcgen05_fence_after();
 			const uint32_t tmem_base = bars.tmem_base;
 			volatile int *abort_flag = &bars.abort_flag;
-			if (!p.after_gated)
+			if (!AFTER_GATED)
 			{ // the next launch may start (and fetch weights) once every CTA is here: all that ran before this launch is then done
 				wait_for_previous_grid();
 				let_next_grid_start();
@@ -193,7 +193,7 @@ namespace mb200
 					};
 					int ahead = 0; // stages whose weights were asked for before the launch ahead was done
 					groups = first_group(1) - g0;
-					if (p.after_gated)
+					if (AFTER_GATED)
 					{
 						for (int kb = kb0; kb < kb1 && ahead < p.stages; kb += p.blocks_per_stage, ahead++)
 							weights(kb, ahead);
@@ -618,7 +618,7 @@ namespace mb200
 			return launch<GATED, decltype(g)::value>(ctx, f, p);
 		});
 	}
-	bool few_product(mlContext_t ctx, const FewTokens &f, int N, __half *y, int ldy, float beta, bool after_gated)
+	bool few_product_after_gated(mlContext_t ctx, const FewTokens &f, int N, __half *y, int ldy, float beta)
 	{
 		Params p;
 		std::memset(&p, 0, sizeof(p));
@@ -626,7 +626,6 @@ namespace mb200
 		p.out = y;
 		p.ldo = ldy;
 		p.beta = beta;
-		p.after_gated = after_gated;
 		return launch<PRODUCT, 0>(ctx, f, p);
 	}
 	int few_statistics_parts(mlContext_t ctx, int N)

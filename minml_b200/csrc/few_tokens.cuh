@@ -20,9 +20,8 @@ namespace mb200
 	};
 	/* h = act(a) u, w = [Wg; Wu]; h has pitch ldh and ldh - hidden columns of padding that are left as they are */
 	bool few_gated(mlContext_t ctx, const FewTokens &p, int hidden, int gate, __half *h, int ldh);
-	/* y [tokens, N] = x w^T + beta y.  `after_gated`: the launch ahead of this one in the stream is few_gated's, under which the first weights are
-	 * fetched. */
-	bool few_product(mlContext_t ctx, const FewTokens &p, int N, __half *y, int ldy, float beta, bool after_gated);
+	/* y [tokens, N] = x w^T + beta y.  The launch ahead of this one in the stream has to be few_gated's: the first weights are fetched under it. */
+	bool few_product_after_gated(mlContext_t ctx, const FewTokens &p, int N, __half *y, int ldy, float beta);
 	/* As pair_statistics (gemm_pair.cuh), with few_statistics_parts(ctx, N) groups of columns */
 	int few_statistics_parts(mlContext_t ctx, int N);
 	bool few_statistics(mlContext_t ctx, const FewTokens &p, int N, const int *targets, float2 *parts, float *target_logit);

@@ -27,12 +27,6 @@ namespace mb200
 	{
 		constexpr float EPSILON = 1.0e-6f; // inside the square root, as in cuda_layernorm_forward
 
-		template<typename T, int VEC>
-		struct alignas(sizeof(T) * VEC) Pack
-		{
-				T v[VEC];
-		};
-
 		/* Sums a and b over the threads of a team of W: a warp by shuffles, several warps through `scratch` (two halves used in turn,
 		 * so one barrier a call is enough: a thread that writes half h again has passed the barrier of the call in between). */
 		template<int W>
@@ -62,39 +56,30 @@ namespace mb200
 			}
 		}
 
-		template<typename T, int VEC, int E>
+		template<typename T, int E>
 		struct RowPart
 		{ // a thread's share of one row, as loaded
-				static constexpr int N = E / VEC;
-				Pack<T, VEC> p[N];
+				T v[E];
 				template<int W>
 				__device__ __forceinline__ void load(const T *row, int lane, int channels)
 				{
 #pragma unroll
-					for (int i = 0; i < N; i++)
+					for (int k = 0; k < E; k++)
 					{
-						const int c = (i * W + lane) * VEC;
-						if (c < channels)
-							p[i] = *reinterpret_cast<const Pack<T, VEC>*>(row + c);
-						else
-						{
-#pragma unroll
-							for (int k = 0; k < VEC; k++)
-								p[i].v[k] = from_float<T>(0.0f);
-						}
+						const int c = k * W + lane;
+						v[k] = c < channels ? row[c] : from_float<T>(0.0f);
 					}
 				}
-				__device__ __forceinline__ float get(int e) const
+				__device__ __forceinline__ float get(int k) const
 				{
-					return to_float(p[e / VEC].v[e % VEC]);
+					return to_float(v[k]);
 				}
 		};
 
-		template<typename T, int VEC, int W, int E>
+		template<typename T, int W, int E>
 		__global__ void __launch_bounds__(W == 32 ? 256 : W) kernel_layernorm_train(T *output, const T *input, const T *ext, const T *__restrict__ gamma,
 				const T *__restrict__ beta, float2 *__restrict__ stats, long long rows, int channels)
 		{
-			constexpr int N = E / VEC;
 			__shared__ float2 scratch[2][16];
 			uint32_t turn = 0;
 			const int lane = threadIdx.x % W;
@@ -102,7 +87,7 @@ namespace mb200
 			const long long teams = static_cast<long long>(gridDim.x) * teams_per_block;
 			for (long long r = static_cast<long long>(blockIdx.x) * teams_per_block + threadIdx.x / W; r < rows; r += teams)
 			{
-				RowPart<T, VEC, E> x, e;
+				RowPart<T, E> x, e;
 				x.template load<W>(input + r * channels, lane, channels);
 				if (ext != nullptr)
 					e.template load<W>(ext + r * channels, lane, channels);
@@ -120,7 +105,7 @@ namespace mb200
 #pragma unroll
 				for (int k = 0; k < E; k++)
 				{
-					const bool inside = (k / VEC * W + lane) * VEC < channels;
+					const bool inside = k * W + lane < channels;
 					v[k] -= mean;
 					var += inside ? v[k] * v[k] : 0.0f;
 				}
@@ -129,30 +114,20 @@ namespace mb200
 				if (lane == 0)
 					stats[r] = make_float2(mean, inv_stddev);
 #pragma unroll
-				for (int i = 0; i < N; i++)
+				for (int k = 0; k < E; k++)
 				{
-					const int c = (i * W + lane) * VEC;
-					if (c >= channels)
-						continue;
-					Pack<T, VEC> g, b, out;
-					if (gamma != nullptr)
-						g = *reinterpret_cast<const Pack<T, VEC>*>(gamma + c);
-					if (beta != nullptr)
-						b = *reinterpret_cast<const Pack<T, VEC>*>(beta + c);
-#pragma unroll
-					for (int k = 0; k < VEC; k++)
-						out.v[k] = from_float<T>((gamma != nullptr ? to_float(g.v[k]) : 1.0f) * v[i * VEC + k] * inv_stddev + (beta != nullptr ? to_float(b.v[k]) : 0.0f));
-					*reinterpret_cast<Pack<T, VEC>*>(output + r * channels + c) = out;
+					const int c = k * W + lane;
+					if (c < channels)
+						output[r * channels + c] = from_float<T>((gamma != nullptr ? to_float(gamma[c]) : 1.0f) * v[k] * inv_stddev + (beta != nullptr ? to_float(beta[c]) : 0.0f));
 				}
 			}
 		}
 
 		/* partial: [2][gridDim.x][channels], the block's column sums of dy xh and of dy */
-		template<typename T, int VEC, int W, int E>
+		template<typename T, int W, int E>
 		__global__ void __launch_bounds__(W == 32 ? 256 : W) kernel_layernorm_backward(T *dx, const T *input, const T *ext, const T *dy,
 				const T *__restrict__ gamma, const float2 *__restrict__ stats, float beta_dx, float *__restrict__ partial, long long rows, int channels)
 		{
-			constexpr int N = E / VEC;
 			__shared__ float2 scratch[2][16];
 			__shared__ float columns[W == 32 ? 7 * 32 * E : 1]; // the other warps' column sums, when a block has eight one-warp teams
 			uint32_t turn = 0;
@@ -161,7 +136,7 @@ namespace mb200
 			const long long teams = static_cast<long long>(gridDim.x) * teams_per_block;
 			const float inv_n = 1.0f / static_cast<float>(channels), inv_n1 = 1.0f / static_cast<float>(channels - 1);
 
-			RowPart<T, VEC, E> g, x, e, d;
+			RowPart<T, E> g, x, e, d;
 			if (gamma != nullptr)
 				g.template load<W>(gamma, lane, channels);
 			float sum_w[E], sum_b[E];
@@ -189,7 +164,7 @@ namespace mb200
 #pragma unroll
 				for (int k = 0; k < E; k++)
 				{
-					const bool inside = (k / VEC * W + lane) * VEC < channels;
+					const bool inside = k * W + lane < channels;
 					const float dv = d.get(k);
 					xh[k] = inside ? (x.get(k) + (ext != nullptr ? e.get(k) : 0.0f) - mean) * inv_stddev : 0.0f;
 					gy[k] = dv * (gamma != nullptr ? g.get(k) : 1.0f);
@@ -204,22 +179,14 @@ namespace mb200
 				s1 *= inv_n;
 				s2 *= inv_n1;
 #pragma unroll
-				for (int i = 0; i < N; i++)
+				for (int k = 0; k < E; k++)
 				{
-					const int c = (i * W + lane) * VEC;
+					const int c = k * W + lane;
 					if (c >= channels)
 						continue;
-					Pack<T, VEC> *dst = reinterpret_cast<Pack<T, VEC>*>(dx + r * channels + c);
-					Pack<T, VEC> out;
-					if (beta_dx != 0.0f)
-						out = *dst;
-#pragma unroll
-					for (int k = 0; k < VEC; k++)
-					{
-						const float v = inv_stddev * (gy[i * VEC + k] - s1 - xh[i * VEC + k] * s2);
-						out.v[k] = from_float<T>(beta_dx != 0.0f ? v + beta_dx * to_float(out.v[k]) : v);
-					}
-					*dst = out;
+					T *dst = dx + r * channels + c;
+					const float v = inv_stddev * (gy[k] - s1 - xh[k] * s2);
+					*dst = from_float<T>(beta_dx != 0.0f ? v + beta_dx * to_float(*dst) : v);
 				}
 			}
 
@@ -257,7 +224,7 @@ namespace mb200
 #pragma unroll
 			for (int k = 0; k < E; k++)
 			{
-				const int c = (k / VEC * W + lane) * VEC + k % VEC;
+				const int c = k * W + lane;
 				if (c < channels)
 				{
 					partial[static_cast<long long>(blockIdx.x) * channels + c] = sum_w[k];
@@ -1017,10 +984,10 @@ namespace mb200
 				done[device] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, RING_BYTES) == cudaSuccess;
 			return done[device];
 		}
-		template<typename T, int VEC, int W, int E>
+		template<typename T, bool WIDE, int W, int E>
 		void launch_team(mlContext_t ctx, cudaStream_t stream, const Args<T> &a, bool backward)
 		{
-			if constexpr (VEC > 1 && W == 32)
+			if constexpr (WIDE && W == 32)
 			{
 				// as many rows at once as the registers hold
 				constexpr int ROWS = 32 / E / (sizeof(T) == 4 ? 2 : 1), FEWER = ROWS > 1 ? ROWS / 2 : 1, BACKWARD_ROWS = E == 8 ? ROWS : 1;
@@ -1034,7 +1001,7 @@ namespace mb200
 				else
 					kernel_layernorm_train_rows<T, E, ROWS, false> <<<a.blocks, threads, 0, stream>>>(a.out, a.x, a.ext, a.gamma, a.beta, a.stats, a.rows, a.channels);
 			}
-			else if constexpr (VEC > 1)
+			else if constexpr (WIDE)
 			{
 				static bool forward_done[MAX_DEVICES] = { }, backward_done[MAX_DEVICES] = { };
 				const int device = get(ctx)->device;
@@ -1060,25 +1027,25 @@ namespace mb200
 							a.status);
 			}
 			else if (backward)
-				kernel_layernorm_backward<T, VEC, W, E> <<<a.blocks, W == 32 ? 256 : W, 0, stream>>>(a.out, a.x, a.ext, a.dy, a.gamma, a.stats, a.beta_dx, a.partial, a.rows, a.channels);
+				kernel_layernorm_backward<T, W, E> <<<a.blocks, W == 32 ? 256 : W, 0, stream>>>(a.out, a.x, a.ext, a.dy, a.gamma, a.stats, a.beta_dx, a.partial, a.rows, a.channels);
 			else
-				kernel_layernorm_train<T, VEC, W, E> <<<a.blocks, W == 32 ? 256 : W, 0, stream>>>(a.out, a.x, a.ext, a.gamma, a.beta, a.stats, a.rows, a.channels);
+				kernel_layernorm_train<T, W, E> <<<a.blocks, W == 32 ? 256 : W, 0, stream>>>(a.out, a.x, a.ext, a.gamma, a.beta, a.stats, a.rows, a.channels);
 		}
-		template<typename T, int VEC>
+		template<typename T, bool WIDE>
 		void launch_by_length(mlContext_t ctx, cudaStream_t stream, const Args<T> &a, bool backward)
 		{
 			if (a.channels <= 32 * 8)
-				launch_team<T, VEC, 32, 8>(ctx, stream, a, backward);
+				launch_team<T, WIDE, 32, 8>(ctx, stream, a, backward);
 			else if (a.channels <= 32 * 16)
-				launch_team<T, VEC, 32, 16>(ctx, stream, a, backward);
+				launch_team<T, WIDE, 32, 16>(ctx, stream, a, backward);
 			else if (a.channels <= 128 * 8)
-				launch_team<T, VEC, 128, 8>(ctx, stream, a, backward);
+				launch_team<T, WIDE, 128, 8>(ctx, stream, a, backward);
 			else if (a.channels <= 128 * 16)
-				launch_team<T, VEC, 128, 16>(ctx, stream, a, backward);
+				launch_team<T, WIDE, 128, 16>(ctx, stream, a, backward);
 			else if (a.channels <= 256 * 16)
-				launch_team<T, VEC, 256, 16>(ctx, stream, a, backward);
+				launch_team<T, WIDE, 256, 16>(ctx, stream, a, backward);
 			else
-				launch_team<T, VEC, 512, 16>(ctx, stream, a, backward);
+				launch_team<T, WIDE, 512, 16>(ctx, stream, a, backward);
 		}
 		/* Through the ring when every row starts on a 16-byte boundary, else element by element into registers */
 		template<typename T>
@@ -1095,9 +1062,9 @@ namespace mb200
 				a.blocks = team_blocks(sms, a.rows, a.channels, wide ? (a.channels <= 512 ? 3 : blocks_per_sm(a.channels)) : a.channels <= 512 ? 8 : a.channels <= 2048 ? 16 : a.channels <= 4096 ? 8 : 4);
 			}
 			if (wide)
-				launch_by_length<T, VEC>(ctx, stream, a, backward);
+				launch_by_length<T, true>(ctx, stream, a, backward);
 			else
-				launch_by_length<T, 1>(ctx, stream, a, backward);
+				launch_by_length<T, false>(ctx, stream, a, backward);
 		}
 
 		template<typename T>
