@@ -298,7 +298,8 @@ void mb200_convolution_forward_noalloc(mlContext_t context, mlDataType_t dtype, 
  * contexts, two replayed graphs) need one each.
  * fp16 and fp32 matrices whose row length is a multiple of 16 bytes must be 16-byte aligned (where they are operands of a product), others
  * are copied to padded rows in the workspace first or, by a forward pass over a few rows, read in place.  No call allocates or synchronises,
- * so each may be captured into a CUDA graph.  Results do not depend on timing (no atomics in sums): the same call gives the same bits.
+ * so each may be captured into a CUDA graph.  Results do not depend on timing (no atomics in sums): the same call gives the same bits.  Rows and
+ * columns are at most 2^31 - 4096, tokens and hidden units of the gated block half of that.
  * fp32 products split their operands (error about that of an fp32 sum): an infinite element may give NaN where fp32 arithmetic gives an
  * infinity. */
 
@@ -314,7 +315,9 @@ void mb200_layernorm_backward(mlContext_t context, const mlTensor_t x, const mlT
 /* Gated feed-forward block: y = (act(x Wg^T) * (x Wu^T)) W2^T + beta * y with W1 = [Wg; Wu], a [2 hidden, embed] matrix (gate rows first), and
  * W2 [embed, hidden].  `gate` names act.  `saved` (optional, fp32 [tokens, 2 hidden]) is where the forward pass may leave what its backward
  * pass reads instead of computing it again; its contents are the library's own.  (For fp16 with embed up to 1024 making most of it again is
- * cheaper, and little of it is used: a caller short of memory loses a tenth of the speed without it.) */
+ * cheaper, and little of it is used: a caller short of memory loses a tenth of the speed without it.)
+ * fp16: act(a) u and the gradients of a and u are rounded to fp16 once, so one above 65504 is an infinity there, also where the result would fit; a
+ * and u themselves are fp32 sums that the tensor core cuts by up to 6.5e-9 of the terms' magnitudes for every index of embed. */
 #define MB200_GATE_SIGMOID 0
 #define MB200_GATE_RELU 1
 #define MB200_GATE_SILU 2
@@ -333,7 +336,8 @@ void mb200_gated_feed_forward_backward(mlContext_t context, const mlTensor_t x, 
 size_t mb200_softmax_cross_entropy_get_workspace_size(mlContext_t context, mlShape_t x_shape, mlShape_t w_shape, mlDataType_t dtype, bool training);
 void mb200_softmax_cross_entropy_forward(mlContext_t context, const mlTensor_t x, const mlTensor_t w, const mlTensor_t targets, mlTensor_t loss, mlTensor_t lse, mlTensor_t workspace);
 /* Gradients of alpha * sum_t row_weights[t] * loss[t] (row_weights optional, fp32 [tokens]), each + beta times its old value; dx, dw are
- * optional.  A row of weight 0 is left out like one without a target.  fp16: choose alpha (the loss scale) so that the gradients fit. */
+ * optional.  A row of weight 0 is left out like one without a target.  fp16: choose alpha (the loss scale) so that the gradients fit; for dw a row of x
+ * is multiplied by its weight over the largest weight and rounded, so a weight less than 2^-14 of the largest costs that row's share digits. */
 void mb200_softmax_cross_entropy_backward(mlContext_t context, const mlTensor_t x, const mlTensor_t w, const mlTensor_t targets, const mlTensor_t lse, float alpha, const mlTensor_t row_weights, float beta_dx, mlTensor_t dx, float beta_dw, mlTensor_t dw, mlTensor_t workspace);
 
 #ifdef __cplusplus

@@ -12,8 +12,9 @@
  *   warp 0 TMA, warp 1 multiplications, warps 2-5 epilogue: a lane is a weight row, so results leave as 64 contiguous bytes a token.
  * Row statistics take an accumulator for every 1024 K indices and add them in fp32, because the tensor core cuts its sums (gemm_pair.cu); those of
  * a tile that do not fit a buffer of tensor memory (embed above 4096 for 64 tokens) come in several.
- * Measured, gated block of 4096 x 11008: 1 token 49 us (two launches, 270 MB: 5.5 TB/s), 64 tokens 61 us.  Above 64 rows the paired kernel
- * (gemm_pair.cu) is as fast or faster: 2048 x 8192, 128 rows 48 us here, 129 rows 39 us there.
+ * Measured, gated block of 4096 x 11008: 1 token 48 us (two launches, 270 MB: 5.6 TB/s), 64 tokens 57 us, where the paired kernel (gemm_pair.cu)
+ * takes 75; 2048 x 8192: 16 tokens 23 us, 48 28 (paired: 35), 64 31 (36).  Logits' statistics, 2048 x 50021: 48 tokens 43 us (47), 64 47 (49).
+ * Above 64 rows, which is what accumulators and epilogue are made for, the paired kernel takes 78 us for 65 and for 96 rows of 4096 x 11008.
  */
 #include "common.cuh"
 #include "tc.cuh"
@@ -493,8 +494,8 @@ namespace mb200
 			}
 		}
 
-		/* CTAs that share a set of rows: enough that each has six boxes to multiply at a time, and a K range of eight blocks.  Measured, 128
-		 * tokens x 4096 x 11008: 83 us with three boxes at least, 72 us with six. */
+		/* CTAs that share a set of rows: enough that each has six boxes to multiply at a time, and a K range of eight blocks.  Measured, 64
+		 * tokens x 4096 x 11008: 61 us with three boxes at least, 57 us with six; 1 token 48.8 and 48.0. */
 		int cluster_size(int sm_count, int boxes, int k_blocks)
 		{
 			int size = 1;

@@ -15,7 +15,8 @@
  * to its split, 700 cycles of one group of warps (two: 2504 -> 2115 us below).  The even CTA issues multiplications that read the lo of B which
  * the odd one's warps wrote, so a split stage is reported with a release at cluster scope, of shared memory alone: of all memory it takes 950
  * cycles more, or 1 200 to 1 400 of a warp that only passes the report on (2205 us -> 2376 below).  Now the tensor core is busy 84 % of the time at 1.44 GHz, the clock under the power limit (4096 x 4096 x 8192).
- * Measured, gated block forward and backward, 2000 x 4001 x 3001: 2085 us (3191 with one CTA a tile), 8192 x 2048 x 8192: 11.0 ms, 225 TFLOP/s.
+ * Measured, gated block forward and backward, 2000 x 4001 x 3001: 2085 - 2450 us by the clock (3191 with one CTA a tile), 8192 x 2048 x 8192: 11.0 -
+ * 12.0 ms, 206 - 225 TFLOP/s.
  */
 #include "common.cuh"
 #include "tc.cuh"
