@@ -381,6 +381,8 @@ class CtypesCalls:
               "softmax_cross_entropy_forward": "tttttw", "softmax_cross_entropy_backward": "ttttntntntw"}
 
     def __getattr__(self, name):
+        if name not in self._FORMS:
+            raise AttributeError(name)
         form, function = self._FORMS[name], getattr(lib, "mb200_" + name)
         tensors = [c for c in form if c in "tw"]
 

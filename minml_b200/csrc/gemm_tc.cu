@@ -56,6 +56,7 @@ namespace mb200
 			record_error(ctx, "cuTensorMapEncodeTiled is not available from the driver");
 			return false;
 		}
+		use_stream(ctx); // the driver encodes for the calling thread's context, and a thread has none before its first runtime call
 		cuuint32_t element_strides[5] = { 1, 1, 1, 1, 1 };
 		cuuint64_t gdims[5];
 		cuuint64_t gstrides[5];
