@@ -317,7 +317,8 @@ void mb200_layernorm_backward(mlContext_t context, const mlTensor_t x, const mlT
  * pass reads instead of computing it again; its contents are the library's own.  (For fp16 with embed up to 1024 making most of it again is
  * cheaper, and little of it is used: a caller short of memory loses a tenth of the speed without it.)
  * fp16: act(a) u and the gradients of a and u are rounded to fp16 once, so one above 65504 is an infinity there, also where the result would fit; a
- * and u themselves are fp32 sums that the tensor core cuts by up to 6.5e-9 of the terms' magnitudes for every index of embed. */
+ * and u themselves are fp32 sums that the tensor core cuts by up to 6.5e-9 of the terms' magnitudes for every index of embed (for up to 64 tokens also
+ * y, for every index of hidden). */
 #define MB200_GATE_SIGMOID 0
 #define MB200_GATE_RELU 1
 #define MB200_GATE_SILU 2
